@@ -12,6 +12,7 @@ columns, weights with one per block of 128 x 128.
 A scale is max(amax of its group, 2^-100) / 448, and q = e4m3(x * 448 / amax): 448 is
 the largest e4m3 value, and the floor keeps the quotients of a group of zeros finite.
 """
+import functools
 import math
 import sys
 from pathlib import Path
@@ -166,7 +167,9 @@ def _plain(state):
     return _as_rows(g / (1 + torch.exp(-g)) * u)
 
 
+@functools.cache
 def _ops():
+    """The framework's operators, imported once as a user's program does."""
     package = str(Path(__file__).resolve().parent.parent / 'dynamic-kv-cache_b200')
     if package not in sys.path:
         sys.path.insert(0, package)
