@@ -27,6 +27,18 @@ cudaError_t launch_silu_mul(const void* gate, const void* up, void* out, int64_t
 cudaError_t launch_add_rms_norm(const void* x, const void* y, void* x_out, void* h_out, const void* weight,
                                 int64_t rows, int width, int64_t xs, int64_t ys, int64_t os, int64_t hs, float eps,
                                 cudaStream_t stream);
+cudaError_t launch_fp8_quantize(const void* x, void* q, float* scale, int64_t rows, int width, int64_t xs,
+                                cudaStream_t stream);
+cudaError_t launch_fp8_quantize_weight(const void* w, void* q, float* scale, int n, int k, int64_t ws,
+                                       cudaStream_t stream);
+cudaError_t launch_add_rms_norm_fp8(const void* x, const void* y, void* x_out, void* q, float* scale,
+                                    const void* weight, int64_t rows, int width, int64_t xs, int64_t ys, int64_t os,
+                                    float eps, cudaStream_t stream);
+cudaError_t launch_fp8_linear(const void* a, const float* sa, const void* w, const float* sw, void* out, int out_f32,
+                              int m, int n, int k, int64_t as, int64_t ws, cudaStream_t stream);
+cudaError_t launch_fp8_gate_up(const void* a, const float* sa, const void* gate, const float* sg, const void* up,
+                               const float* su, void* out, float* out_scale, int m, int n, int k, int64_t as,
+                               int64_t gs, int64_t us, cudaStream_t stream);
 cudaError_t launch_pack_many(const void* k, const void* v, const dkv_pack_target* targets, bool on_device, int count,
                              int64_t kh, int64_t kt, int64_t vh, int64_t vt, int64_t kc, int64_t vc, int layer, int n,
                              int heads, int blocks, cudaStream_t stream);
@@ -595,6 +607,107 @@ int dkv_add_rms_norm(const void* x, const void* y, void* x_out, void* h_out, con
                     cuda_status(dkv::launch_add_rms_norm(x, y, x_out, h_out, weight, rows, width, xs, ys, os, hs, eps,
                                                          static_cast<cudaStream_t>(stream)),
                                 "add_rms_norm launch"));
+}
+
+// Widths of 8-bit rows: a multiple of 16 (rows begin 16 bytes apart), at most 16384.
+static int check_fp8_width(const char* what, int32_t width) {
+  if (width <= 0 || width % 16 || width > 16384)
+    return fail(DKV_EINVAL, "%s: width must be a multiple of 16 in [16, 16384]", what);
+  return DKV_OK;
+}
+
+static bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+int dkv_fp8_quantize(const void* x, void* q, float* scale, int64_t rows, int32_t width, int64_t xs, void* stream) {
+  int rc = check_fp8_width("fp8_quantize", width);
+  if (rc) return rc;
+  if (rows < 0) return fail(DKV_EINVAL, "fp8_quantize: negative row count");
+  if (rows == 0) return ok();
+  if (!x || !q || !scale) return fail(DKV_EINVAL, "fp8_quantize: null pointer");
+  if (!aligned16(x) || !aligned16(q) || !aligned4(scale))
+    return fail(DKV_EINVAL, "fp8_quantize: tensors must be 16-byte aligned");
+  if (xs < width || xs % 8) return fail(DKV_EINVAL, "fp8_quantize: row strides must hold a row and be multiples of 8 elements");
+  if (rows > INT32_MAX / ((width + 127) / 128)) return fail(DKV_EINVAL, "fp8_quantize: too many rows");
+  return note_write(stream, kWroteNothing,
+                    cuda_status(dkv::launch_fp8_quantize(x, q, scale, rows, width, xs, static_cast<cudaStream_t>(stream)),
+                                "fp8_quantize launch"));
+}
+
+int dkv_fp8_quantize_weight(const void* w, void* q, float* scale, int32_t n, int32_t k, int64_t ws, void* stream) {
+  int rc = check_fp8_width("fp8_quantize_weight", k);
+  if (rc) return rc;
+  if (n <= 0 || n > (1 << 24)) return fail(DKV_EINVAL, "fp8_quantize_weight: 1 to 2^24 rows");
+  if (!w || !q || !scale) return fail(DKV_EINVAL, "fp8_quantize_weight: null pointer");
+  if (!aligned16(w) || !aligned16(q) || !aligned4(scale))
+    return fail(DKV_EINVAL, "fp8_quantize_weight: tensors must be 16-byte aligned");
+  if (ws < k || ws % 8)
+    return fail(DKV_EINVAL, "fp8_quantize_weight: row strides must hold a row and be multiples of 8 elements");
+  return note_write(stream, kWroteNothing,
+                    cuda_status(dkv::launch_fp8_quantize_weight(w, q, scale, n, k, ws, static_cast<cudaStream_t>(stream)),
+                                "fp8_quantize_weight launch"));
+}
+
+int dkv_add_rms_norm_fp8(const void* x, const void* y, void* x_out, void* q, float* scale, const void* weight,
+                         int64_t rows, int32_t width, int64_t xs, int64_t ys, int64_t os, float eps, void* stream) {
+  int rc = check_fp8_width("add_rms_norm_fp8", width);
+  if (rc) return rc;
+  if (rows < 0) return fail(DKV_EINVAL, "add_rms_norm_fp8: negative row count");
+  if (!(eps >= 0.f)) return fail(DKV_EINVAL, "add_rms_norm_fp8: eps must be non-negative");
+  if (rows == 0) return ok();
+  if (!x || !q || !scale || !weight || (y != nullptr && x_out == nullptr))
+    return fail(DKV_EINVAL, "add_rms_norm_fp8: null pointer");
+  if (!aligned16(x) || !aligned16(q) || !aligned4(scale) || !aligned16(weight) ||
+      (y && (!aligned16(y) || !aligned16(x_out))))
+    return fail(DKV_EINVAL, "add_rms_norm_fp8: tensors must be 16-byte aligned");
+  if (xs < width || xs % 8 || (y && (ys < width || os < width || ys % 8 || os % 8)))
+    return fail(DKV_EINVAL, "add_rms_norm_fp8: row strides must hold a row and be multiples of 8 elements");
+  if (rows > INT32_MAX) return fail(DKV_EINVAL, "add_rms_norm_fp8: too many rows");
+  return note_write(stream, kWroteNothing,
+                    cuda_status(dkv::launch_add_rms_norm_fp8(x, y, x_out, q, scale, weight, rows, width, xs, ys, os, eps,
+                                                             static_cast<cudaStream_t>(stream)),
+                                "add_rms_norm_fp8 launch"));
+}
+
+int dkv_fp8_linear(const void* a, const float* a_scale, const void* w, const float* w_scale, void* out,
+                   int32_t out_bits, int64_t m, int32_t n, int32_t k, int64_t as, int64_t ws, void* stream) {
+  int rc = check_fp8_width("fp8_linear", k);
+  if (rc) return rc;
+  if (out_bits != 16 && out_bits != 32) return fail(DKV_EINVAL, "fp8_linear: out is bf16 (16) or fp32 (32)");
+  if (m < 0 || m > (1 << 21)) return fail(DKV_EINVAL, "fp8_linear: 0 to 2^21 rows");
+  if (n <= 0 || n > (1 << 24)) return fail(DKV_EINVAL, "fp8_linear: 1 to 2^24 weight rows");
+  if (m == 0) return ok();
+  if (!a || !a_scale || !w || !w_scale || !out) return fail(DKV_EINVAL, "fp8_linear: null pointer");
+  if (!aligned16(a) || !aligned16(w) || !aligned16(out) || !aligned4(a_scale) || !aligned4(w_scale))
+    return fail(DKV_EINVAL, "fp8_linear: tensors must be 16-byte aligned");
+  if (as < k || ws < k || as % 16 || ws % 16)
+    return fail(DKV_EINVAL, "fp8_linear: row strides must hold a row and be multiples of 16 bytes");
+  return note_write(stream, kWroteNothing,
+                    cuda_status(dkv::launch_fp8_linear(a, a_scale, w, w_scale, out, out_bits == 32,
+                                                       static_cast<int>(m), n, k, as, ws,
+                                                       static_cast<cudaStream_t>(stream)),
+                                "fp8_linear launch"));
+}
+
+int dkv_fp8_gate_up(const void* a, const float* a_scale, const void* gate, const float* gate_scale, const void* up,
+                    const float* up_scale, void* q, float* scale, int64_t m, int32_t n, int32_t k, int64_t as,
+                    int64_t gs, int64_t us, void* stream) {
+  int rc = check_fp8_width("fp8_gate_up", k);
+  if (rc) return rc;
+  if ((rc = check_fp8_width("fp8_gate_up output", n))) return rc;
+  if (m < 0 || m > (1 << 21)) return fail(DKV_EINVAL, "fp8_gate_up: 0 to 2^21 rows");
+  if (m == 0) return ok();
+  if (!a || !a_scale || !gate || !gate_scale || !up || !up_scale || !q || !scale)
+    return fail(DKV_EINVAL, "fp8_gate_up: null pointer");
+  if (!aligned16(a) || !aligned16(gate) || !aligned16(up) || !aligned16(q) || !aligned4(a_scale) ||
+      !aligned4(gate_scale) || !aligned4(up_scale) || !aligned4(scale))
+    return fail(DKV_EINVAL, "fp8_gate_up: tensors must be 16-byte aligned");
+  if (as < k || gs < k || us < k || as % 16 || gs % 16 || us % 16)
+    return fail(DKV_EINVAL, "fp8_gate_up: row strides must hold a row and be multiples of 16 bytes");
+  return note_write(stream, kWroteNothing,
+                    cuda_status(dkv::launch_fp8_gate_up(a, a_scale, gate, gate_scale, up, up_scale, q, scale,
+                                                        static_cast<int>(m), n, k, as, gs, us,
+                                                        static_cast<cudaStream_t>(stream)),
+                                "fp8_gate_up launch"));
 }
 
 }  // extern "C"

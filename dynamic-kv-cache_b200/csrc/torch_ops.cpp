@@ -12,6 +12,7 @@
 #include <map>
 #include <mutex>
 #include <stdexcept>
+#include <string>
 #include <utility>
 #include <vector>
 
@@ -173,6 +174,169 @@ std::vector<at::Tensor> add_rms_norm(const at::Tensor& x_in, const c10::optional
   return {x_out, h};
 }
 
+// -- 8-bit decoder operators (dkv_fp8_*): e4m3 codes and fp32 scales ------------------
+
+namespace {
+
+constexpr int64_t kGroup = 128;
+
+int64_t groups_of(int64_t width) { return (width + kGroup - 1) / kGroup; }
+
+// The operators have no backward pass: a call that autograd would have to follow is refused.
+void no_grad(const at::Tensor& x, const char* what) {
+  if (x.requires_grad() && at::GradMode::is_enabled())
+    throw pybind11::value_error(std::string(what) + " has no backward pass (call it under torch.no_grad())");
+}
+
+// bf16 [..., width] as rows the kernels can load 16 bytes at a time; `stride` receives
+// the row stride in elements.
+at::Tensor bf16_rows(const at::Tensor& x, const char* what, int64_t* stride) {
+  if (!x.is_cuda() || x.scalar_type() != at::kBFloat16 || x.dim() < 1)
+    throw pybind11::value_error(std::string(what) + " takes CUDA bfloat16 tensors");
+  no_grad(x, what);
+  const int64_t width = x.size(-1);
+  if (x.dim() == 2 && x.size(0) > 0 && x.stride(1) == 1 && x.stride(0) >= width && x.stride(0) % 8 == 0 &&
+      (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15u) == 0) {
+    *stride = x.stride(0);
+    return x;
+  }
+  *stride = width;
+  const at::Tensor c = x.contiguous();
+  return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) == 0 ? c : c.clone();
+}
+
+// e4m3 matrix [..., width] of 16-byte aligned rows; `stride` receives the row stride in bytes.
+at::Tensor e4m3_rows(const at::Tensor& q, const char* what, int64_t* stride) {
+  if (!q.is_cuda() || q.scalar_type() != at::kFloat8_e4m3fn || q.dim() < 1)
+    throw pybind11::value_error(std::string(what) + " takes CUDA float8_e4m3fn codes");
+  const int64_t width = q.size(-1);
+  if (q.dim() == 2 && q.size(0) > 0 && q.stride(1) == 1 && q.stride(0) >= width && q.stride(0) % 16 == 0 &&
+      (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15u) == 0) {
+    *stride = q.stride(0);
+    return q;
+  }
+  *stride = width;
+  const at::Tensor c = q.contiguous();
+  return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) == 0 ? c : c.clone();
+}
+
+// The scales of e4m3 rows [..., width]: fp32 [..., groups], contiguous.
+at::Tensor row_scales(const at::Tensor& s, const at::Tensor& q, const char* what) {
+  bool ok = s.scalar_type() == at::kFloat && s.device() == q.device() && s.dim() == q.dim() &&
+            s.size(-1) == groups_of(q.size(-1));
+  for (int64_t d = 0; ok && d + 1 < q.dim(); ++d) ok = s.size(d) == q.size(d);
+  if (!ok) throw pybind11::value_error(std::string(what) + ": rows need fp32 scales [..., ceil(width / 128)] on their device");
+  return s.contiguous();
+}
+
+// The scales of e4m3 weights [n, k]: fp32 [ceil(n / 128), ceil(k / 128)], contiguous.
+at::Tensor block_scales(const at::Tensor& s, const at::Tensor& q, const char* what) {
+  if (q.dim() != 2 || s.dim() != 2 || s.scalar_type() != at::kFloat || s.device() != q.device() ||
+      s.size(0) != groups_of(q.size(0)) || s.size(1) != groups_of(q.size(1)))
+    throw pybind11::value_error(std::string(what) +
+                                ": weights are [n, k] with fp32 scales [ceil(n / 128), ceil(k / 128)] on their device");
+  return s.contiguous();
+}
+
+std::vector<int64_t> with_last(const at::Tensor& x, int64_t last) {
+  std::vector<int64_t> sizes = x.sizes().vec();
+  sizes.back() = last;
+  return sizes;
+}
+
+int64_t rows_of(const at::Tensor& x) { return x.size(-1) ? x.numel() / x.size(-1) : 0; }
+
+int32_t narrow(int64_t v) { return v > INT32_MAX ? INT32_MAX : static_cast<int32_t>(v); }
+
+float* fp(const at::Tensor& t) { return static_cast<float*>(t.data_ptr()); }
+
+}  // namespace
+
+// bf16 rows x [..., width] to (codes [..., width], scales [..., ceil(width / 128)]).
+std::vector<at::Tensor> fp8_quantize(const at::Tensor& x_in) {
+  int64_t xs;
+  const at::Tensor x = bf16_rows(x_in, "fp8_quantize", &xs);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t width = x.size(-1);
+  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor s = at::empty(with_last(x, groups_of(width)), x.options().dtype(at::kFloat));
+  check(dkv_fp8_quantize(x.data_ptr(), q.data_ptr(), fp(s), rows_of(x), narrow(width), xs, current_stream(x)));
+  return {q, s};
+}
+
+// bf16 weights w [n, k] to (codes [n, k], scales [ceil(n / 128), ceil(k / 128)]).
+std::vector<at::Tensor> fp8_quantize_weight(const at::Tensor& w_in) {
+  if (w_in.dim() != 2) throw pybind11::value_error("fp8_quantize_weight takes weights [n, k]");
+  int64_t ws;
+  const at::Tensor w = bf16_rows(w_in, "fp8_quantize_weight", &ws);
+  const c10::cuda::CUDAGuard guard(w.device());
+  const int64_t n = w.size(0), k = w.size(1);
+  at::Tensor q = at::empty({n, k}, w.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor s = at::empty({groups_of(n), groups_of(k)}, w.options().dtype(at::kFloat));
+  check(dkv_fp8_quantize_weight(w.data_ptr(), q.data_ptr(), fp(s), narrow(n), narrow(k), ws, current_stream(w)));
+  return {q, s};
+}
+
+// (x + y, codes, scales of its norm) over the rows of x / y [..., width]; (x, ...) without y.
+std::vector<at::Tensor> add_rms_norm_fp8(const at::Tensor& x_in, const c10::optional<at::Tensor>& y_in,
+                                         const at::Tensor& weight_in, double eps) {
+  int64_t xs, ys = 0, wstride;
+  const at::Tensor x = bf16_rows(x_in, "add_rms_norm_fp8", &xs);
+  const int64_t width = x.size(-1);
+  if (weight_in.dim() != 1 || weight_in.size(0) != width || weight_in.device() != x.device())
+    throw pybind11::value_error("add_rms_norm_fp8: weight must be [width]");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const at::Tensor w = bf16_rows(weight_in, "add_rms_norm_fp8", &wstride);
+  at::Tensor y, x_out = x_in;
+  if (y_in.has_value()) {
+    if (y_in->sizes() != x.sizes() || y_in->device() != x.device())
+      throw pybind11::value_error("add_rms_norm_fp8: y must match x");
+    y = bf16_rows(*y_in, "add_rms_norm_fp8", &ys);
+    x_out = at::empty(x.sizes(), x.options());
+  }
+  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor s = at::empty(with_last(x, groups_of(width)), x.options().dtype(at::kFloat));
+  check(dkv_add_rms_norm_fp8(x.data_ptr(), y.defined() ? y.data_ptr() : nullptr,
+                             y.defined() ? x_out.data_ptr() : nullptr, q.data_ptr(), fp(s), w.data_ptr(), rows_of(x),
+                             narrow(width), xs, ys, width, static_cast<float>(eps), current_stream(x)));
+  return {x_out, q, s};
+}
+
+// The linear layer of e4m3 rows (q, s) [..., k] and e4m3 weights (w, ws) [n, k]: [..., n] in bf16 or fp32.
+at::Tensor fp8_linear(const at::Tensor& q_in, const at::Tensor& s_in, const at::Tensor& w_in, const at::Tensor& ws_in,
+                      bool out_f32) {
+  int64_t as, wstride;
+  const at::Tensor q = e4m3_rows(q_in, "fp8_linear", &as), w = e4m3_rows(w_in, "fp8_linear", &wstride);
+  const at::Tensor s = row_scales(s_in, q, "fp8_linear"), wsc = block_scales(ws_in, w, "fp8_linear");
+  if (w.device() != q.device() || w.size(1) != q.size(-1))
+    throw pybind11::value_error("fp8_linear: rows and weights must share their device and width");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int64_t n = w.size(0), k = w.size(1);
+  at::Tensor out = at::empty(with_last(q, n), q.options().dtype(out_f32 ? at::kFloat : at::kBFloat16));
+  check(dkv_fp8_linear(q.data_ptr(), fp(s), w.data_ptr(), fp(wsc), out.data_ptr(), out_f32 ? 32 : 16, rows_of(q),
+                       narrow(n), narrow(k), as, wstride, current_stream(q)));
+  return out;
+}
+
+// silu(rows gate^T) * (rows up^T) as (codes [..., n], scales [..., ceil(n / 128)]).
+std::vector<at::Tensor> fp8_gate_up(const at::Tensor& q_in, const at::Tensor& s_in, const at::Tensor& g_in,
+                                    const at::Tensor& gs_in, const at::Tensor& u_in, const at::Tensor& us_in) {
+  int64_t as, gstride, ustride;
+  const at::Tensor q = e4m3_rows(q_in, "fp8_gate_up", &as), g = e4m3_rows(g_in, "fp8_gate_up", &gstride),
+                   u = e4m3_rows(u_in, "fp8_gate_up", &ustride);
+  const at::Tensor s = row_scales(s_in, q, "fp8_gate_up");
+  const at::Tensor gsc = block_scales(gs_in, g, "fp8_gate_up"), usc = block_scales(us_in, u, "fp8_gate_up");
+  if (g.device() != q.device() || u.device() != q.device() || g.sizes() != u.sizes() || g.size(1) != q.size(-1))
+    throw pybind11::value_error("fp8_gate_up: gate and up must have one shape [n, width] on the rows' device");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int64_t n = g.size(0), k = g.size(1);
+  at::Tensor out = at::empty(with_last(q, n), q.options());
+  at::Tensor scale = at::empty(with_last(q, groups_of(n)), s.options());
+  check(dkv_fp8_gate_up(q.data_ptr(), fp(s), g.data_ptr(), fp(gsc), u.data_ptr(), fp(usc), out.data_ptr(), fp(scale),
+                        rows_of(q), narrow(n), narrow(k), as, gstride, ustride, current_stream(q)));
+  return {out, scale};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "C++ host path of GPUCache's per-layer calls into libdkv.so";
   m.def("workspace", &workspace);
@@ -180,4 +344,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pack", &pack);
   m.def("append_attend", &append_attend);
   m.def("add_rms_norm", &add_rms_norm);
+  m.def("fp8_quantize", &fp8_quantize);
+  m.def("fp8_quantize_weight", &fp8_quantize_weight);
+  m.def("add_rms_norm_fp8", &add_rms_norm_fp8);
+  m.def("fp8_linear", &fp8_linear);
+  m.def("fp8_gate_up", &fp8_gate_up);
 }

@@ -9,6 +9,7 @@ and the weight-joining invariants (bit-identical parameter views over one joined
 tensor) are the same.
 """
 import types
+from typing import NamedTuple
 
 import torch
 
@@ -42,6 +43,51 @@ def activation_product(gate, up):
     if gate.is_cuda and gate.dtype == torch.bfloat16 and up.dtype == torch.bfloat16 and gate.shape == up.shape:
         return K.silu_mul(gate, up)
     return torch.nn.functional.silu(gate) * up
+
+
+# -- 8-bit projections (dkv_fp8_*; not in the reference) ---------------------------
+# e4m3 codes with fp32 scales: activations one scale per row and group of 128
+# columns, weights one per block of 128 x 128 (scale = amax / 448, include/dkv.h).
+# CUDA only, widths multiples of 16, no backward pass. Sums stay in fp32 and each
+# result is rounded once; a NaN or infinity in a group makes its products NaN.
+
+class Fp8(NamedTuple):
+    """8-bit rows or weights: float8_e4m3fn codes and their fp32 scales."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+
+def fp8_quantize(x):
+    """bf16 rows x [..., width] as Fp8(codes [..., width], scales [..., ceil(width / 128)])."""
+    return Fp8(*K.FAST.fp8_quantize(x))
+
+
+def fp8_quantize_weight(w):
+    """bf16 weights w [n, k] as Fp8(codes [n, k], scales [ceil(n / 128), ceil(k / 128)]): once per weight."""
+    return Fp8(*K.FAST.fp8_quantize_weight(w))
+
+
+def add_rms_fp8(x, y, weight, eps):
+    """add_rms with the normed rows in 8 bits: (x + y, Fp8 rows of RMSNorm(x + y) * weight),
+    or (x, Fp8 rows of RMSNorm(x) * weight) when y is None. The sum is bf16, as add_rms
+    returns it; the norm is of that sum and stays in fp32 until its rounding to 8 bits."""
+    out, q, scale = K.FAST.add_rms_norm_fp8(x, y, weight, eps)
+    return out, Fp8(q, scale)
+
+
+def fp8_linear(a, w, dtype=torch.bfloat16):
+    """The linear layer a w^T of 8-bit rows a [..., k] (fp8_quantize, add_rms_fp8, fp8_gate_up)
+    and 8-bit weights w [n, k] (fp8_quantize_weight): [..., n] in bf16 or fp32."""
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError('fp8_linear returns bfloat16 or float32')
+    return K.FAST.fp8_linear(a[0], a[1], w[0], w[1], dtype == torch.float32)
+
+
+def fp8_gate_up(a, gate, up):
+    """silu(a gate^T) * (a up^T) as Fp8 rows [..., n], for 8-bit rows a [..., k] and 8-bit
+    weights gate and up [n, k]: both projections, the activation, the product and its
+    rounding to 8 bits in one launch (the input of the down projection)."""
+    return Fp8(*K.FAST.fp8_gate_up(a[0], a[1], gate[0], gate[1], up[0], up[1]))
 
 
 def join_weights(modules):

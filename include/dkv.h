@@ -444,6 +444,62 @@ int dkv_silu_mul(const void* gate, const void* up, void* out, int64_t gs, int64_
 int dkv_add_rms_norm(const void* x, const void* y, void* x_out, void* h_out, const void* weight, int64_t rows,
                      int32_t width, int64_t xs, int64_t ys, int64_t os, int64_t hs, float eps, void* stream);
 
+/*
+ * ---- 8-bit decoder operators (no reference counterpart) ----
+ * The projections around the packed attention in 8 bits: activations are e4m3 rows
+ * with one fp32 scale per row and group of 128 columns, weights e4m3 with one fp32
+ * scale per block of 128 x 128. For a group of values x, amax = max(max |x|, 2^-100),
+ *   scale = amax / 448,   code = e4m3(x * (448 / amax))   (round to nearest even)
+ * and the group stands for code * scale. A NaN makes its group's scale NaN, an
+ * infinity makes it infinite; every product with that group is then NaN. Widths are
+ * multiples of 16 (at most 16384); the last group of a row, and the last block of
+ * weight rows, may be partial. q / scale of a call are contiguous unless a stride is
+ * given; row strides of 8-bit matrices are in bytes, multiples of 16. Input and output
+ * tensors of one call must not overlap. 16-byte aligned tensors (scales: 4). Nothing
+ * here needs a workspace; every entry point may be captured into a CUDA graph.
+ */
+
+/* bf16 rows to e4m3 rows: x [rows, width] (row stride xs elements, a multiple of 8) ->
+ * q [rows, width], scale [rows, ceil(width / 128)]. */
+int dkv_fp8_quantize(const void* x, void* q, float* scale, int64_t rows, int32_t width, int64_t xs, void* stream);
+
+/* bf16 weights to e4m3 blocks (once per weight): w [n, k] (row stride ws elements, a
+ * multiple of 8) -> q [n, k], scale [ceil(n / 128), ceil(k / 128)]. */
+int dkv_fp8_quantize_weight(const void* w, void* q, float* scale, int32_t n, int32_t k, int64_t ws, void* stream);
+
+/*
+ * dkv_add_rms_norm with the normed rows in 8 bits, for the projection that reads them:
+ * x_out = bf16(x + y), then e4m3 rows (q, scale as in dkv_fp8_quantize) of
+ * h = x_out * rsqrt(mean(x_out^2) + eps) * weight, which stays in fp32 until its one
+ * rounding. With y == NULL there is no add and the norm is of x (x_out unused). bf16
+ * x / y / x_out with row strides xs / ys / os in elements (multiples of 8), weight bf16
+ * [width] contiguous.
+ */
+int dkv_add_rms_norm_fp8(const void* x, const void* y, void* x_out, void* q, float* scale, const void* weight,
+                         int64_t rows, int32_t width, int64_t xs, int64_t ys, int64_t os, float eps, void* stream);
+
+/*
+ * out[m, n] = sum over column groups b of a_scale[m, b] * w_scale[n / 128, b] *
+ * sum_{k in b} a[m, k] w[n, k]: the linear layer a w^T of e4m3 rows a [m, k] (row
+ * stride as bytes, a_scale [m, ceil(k / 128)]) and e4m3 weights w [n, k] (row stride
+ * ws bytes, w_scale [ceil(n / 128), ceil(k / 128)]). Sums are fp32, rounded once to
+ * out [m, n], contiguous: bf16 (out_bits 16) or fp32 (32). Deterministic: the same
+ * shape gives the same order of additions.
+ */
+int dkv_fp8_linear(const void* a, const float* a_scale, const void* w, const float* w_scale, void* out,
+                   int32_t out_bits, int64_t m, int32_t n, int32_t k, int64_t as, int64_t ws, void* stream);
+
+/*
+ * The gate and up projections of a decoder MLP, their activation and its rounding to 8
+ * bits in one launch: h = silu(a gate^T) * (a up^T), in fp32 from the sums of both
+ * products to its one rounding, as e4m3 rows q [m, n], scale [m, ceil(n / 128)] (what
+ * the down projection reads). gate and up are e4m3 weights [n, k] with row strides gs /
+ * us in bytes; n is a multiple of 16 (at most 16384).
+ */
+int dkv_fp8_gate_up(const void* a, const float* a_scale, const void* gate, const float* gate_scale, const void* up,
+                    const float* up_scale, void* q, float* scale, int64_t m, int32_t n, int32_t k, int64_t as,
+                    int64_t gs, int64_t us, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
