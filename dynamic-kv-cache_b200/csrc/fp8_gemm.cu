@@ -61,7 +61,15 @@ struct GemmTile {
   }
 };
 
-__device__ __forceinline__ float silu_times(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) * u = g / (1 + 2^(-g log2 e)) * u on the special-function unit: 2^x and 1 / x are off
+// by a few fp32 units, and the exponent's rounding by |g| of them, far under the 2^-4 of the
+// rounding to e4m3 that follows (IEEE expf and division made the epilogue the bottleneck).
+// Where 2^x overflows, 1 / inf = 0 and the result is the 0 that silu tends to.
+__device__ __forceinline__ float silu_times(float g, float u) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(1.0f + ex2(-1.4426950408889634f * g)));
+  return g * r * u;
+}
 
 template <int NT, bool GATE>
 __global__ void __launch_bounds__(kGemmThreads, 1)
@@ -273,6 +281,301 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   if (a.splits > 1) cluster_sync_all();  // the other blocks may still be reading this one's partial sums
 }
 
+// ---- many tokens -----------------------------------------------------------------
+// fp8_wide_kernel keeps the tensor cores busy when there are tokens for it: a pair of
+// blocks works on a tile of 256 tokens x 256 weight rows, each block with 128 of the
+// tokens on its accumulators' lanes and half of the weight rows in its shared memory (so
+// per group and block 32 KB arrive for 2 x 128 x 256 x 128 products). A group's products go
+// to two accumulators of 128 columns, one per weight block of 128 rows; TMEM holds four, so
+// the tensor cores run up to two groups ahead of the eight epilogue warps that scale and
+// add them. A thread owns one token and 64 columns of each half: a half costs it one scale
+// product and 32 packed FMAs. The grid is persistent (one pair per two SMs): a tile's store
+// overlaps the next tile's first groups.
+// GATE makes the halves the gate and the up rows of the same 128 intermediate columns:
+// each thread then holds matching columns of G and U.
+constexpr int kWideThreads = 384;  // warps 0-7: scale and add; 8: copies; 9: MMA issue; 10, 11: none
+constexpr int kWideStages = 6;
+constexpr int kWideHalf = 128 * kFp8Group;  // bytes of one block's operand tile of one group
+constexpr int kWideStageBytes = 2 * kWideHalf;
+constexpr int kWideChunk = 16;  // groups whose scales are staged at a time
+constexpr int kWideScales = kWideChunk * 128 + 2 * kWideChunk;  // [group][token], then [group][half] of the weights
+constexpr int kWideSmem = 1024 + kWideStages * kWideStageBytes + 2 * kWideScales * 4;
+constexpr int kWideCols = 256;
+constexpr int kWideSlots = 2;
+constexpr uint32_t kWideTmem = kWideSlots * kWideCols;
+
+// `count` columns of one token (a multiple of 16), of which `columns` exist.
+__device__ __forceinline__ void store_columns_bf16(__nv_bfloat16* p, int columns, bool vector, const float* v, int count) {
+  if (vector && columns >= count) {
+#pragma unroll
+    for (int j = 0; j < count; j += 16) {
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = __uint_as_float(pack_bf16x2(v[j + 2 * i], v[j + 2 * i + 1]));
+      st_global_v8(reinterpret_cast<float*>(p + j), w);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < count; ++j)
+      if (j < columns) p[j] = __float2bfloat16_rn(v[j]);
+  }
+}
+
+__device__ __forceinline__ void store_columns_f32(float* p, int columns, bool vector, const float* v, int count) {
+  if (vector && columns >= count) {
+#pragma unroll
+    for (int j = 0; j < count; j += 8) st_global_v8(p + j, v + j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < count; ++j)
+      if (j < columns) p[j] = v[j];
+  }
+}
+
+template <bool GATE>
+__global__ void __launch_bounds__(kWideThreads, 1)
+fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap umap,
+                const __grid_constant__ CUtensorMap amap, const GemmArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[2 * kWideStages + kWideSlots + 4];
+  __shared__ uint32_t tmem_slot;
+  __shared__ float amax_part[2][2][128];  // GATE: [tile parity][column part][token]
+  const uint32_t ring = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  const uint32_t full = smem_addr(bars);         // rank 0's: both blocks' copies of a stage
+  // each block's own: a stage's products are done, its accumulator complete and its buffers
+  // empty (one commit for both: a commit costs the issuing thread ~0.15 us)
+  const uint32_t done = full + 8 * kWideStages;
+  const uint32_t freed = done + 8 * kWideStages;  // rank 0's: both blocks have read an accumulator
+  const uint32_t staged = freed + 8 * kWideSlots;  // each block's own: a chunk of scales is there
+  const uint32_t used = staged + 16;               // ... and no longer needed
+  float* const scales = reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)) + kWideStages * kWideStageBytes);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & 1;
+  const int pair = blockIdx.x >> 1;
+  const int pairs = gridDim.x >> 1;
+  constexpr int kColumns = GATE ? 128 : 256;  // output columns of a tile
+  const int tiles_m = (a.m + 255) / 256;
+  const int tiles = tiles_m * ((a.n + kColumns - 1) / kColumns);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2 * kWideStages; ++i) mbar_init(full + 8 * i, 1);
+    for (int i = 0; i < kWideSlots; ++i) mbar_init(freed + 8 * i, 8 + (rank == 0));  // the epilogue warps of both blocks
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(staged + 8 * i, 64);
+      mbar_init(used + 8 * i, 8);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 8 && lane == 0) {
+    prefetch_tensor_map(&wmap);
+    if (GATE) prefetch_tensor_map(&umap);
+    prefetch_tensor_map(&amap);
+  }
+  cluster_sync_all();  // both blocks' barriers exist
+  pdl_wait();
+  if (warp == 9) {  // after the wait, before the trigger: see fp8_gemm_kernel
+    tmem_alloc_pair(smem_addr(&tmem_slot), kWideTmem);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_arrive_release();  // the copies need not wait for TMEM: their warps join at the end
+
+  // 384 x 168 registers at launch = 128 x (56 + 224 + 224)
+  if (warp >= 8) {
+    regs_give<56>();
+    if (warp == 9) {
+      cluster_wait_acquire();
+      tc_fence_after();
+      pdl_trigger();  // after every block's allocation
+    }
+    if (warp == 8 && lane == 0) {
+      const uint32_t full0 = dsmem_addr(full, 0);
+      int i = 0;
+      bool ok = true;
+      for (int tile = pair; tile < tiles && ok; tile += pairs) {
+        const int token0 = (tile % tiles_m) * 256 + rank * 128;
+        const int row0 = (tile / tiles_m) * kColumns + (GATE ? 0 : rank * 128);
+        for (int g = 0; g < a.groups; ++g, ++i) {
+          const int s = i % kWideStages;
+          if (i >= kWideStages && !mbar_wait(done + 8 * s, ((i / kWideStages) + 1) & 1, kGemmWaitCycles)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = ring + s * kWideStageBytes;
+          if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, 2 * kWideStageBytes);
+          tile2d_g2s_pair(dst, &amap, g * kFp8Group, token0, full0 + 8 * s);
+          tile2d_g2s_pair(dst + kWideHalf, GATE && rank == 1 ? &umap : &wmap, g * kFp8Group, row0, full0 + 8 * s);
+        }
+      }
+      if (!ok && rank == 0)  // a wait that ran out: the copies in flight still target shared memory
+        for (int j = max(0, i - kWideStages); j < i; ++j)
+          mbar_wait(full + 8 * (j % kWideStages), (j / kWideStages) & 1, kGemmWaitCycles);
+    } else if (warp == 9 && rank == 1 && lane == 0) {
+      const int total = (tiles - pair + pairs - 1) / pairs * a.groups;
+      const uint32_t freed0 = dsmem_addr(freed, 0);
+      for (int i = 0; i < total; ++i) {
+        const int slot = i % kWideSlots;
+        if (!mbar_wait(freed + 8 * slot, (i / kWideSlots) & 1, kGemmWaitCycles)) break;
+        mbar_arrive_cluster(freed0 + 8 * slot);
+      }
+    } else if (warp == 9 && rank == 0 && lane == 0) {
+      constexpr uint32_t idesc = idesc_e4m3(256, kWideCols);
+      const uint32_t tmem = tmem_slot;
+      const int total = (tiles - pair + pairs - 1) / pairs * a.groups;
+      bool ok = true;
+      for (int i = 0; i < total && ok; ++i) {
+        const int s = i % kWideStages;
+        ok = mbar_wait(full + 8 * s, (i / kWideStages) & 1, kGemmWaitCycles);
+        const uint32_t src = ring + s * kWideStageBytes;
+        const uint64_t ad = sw128_desc(src, 16, 1024);
+        const uint64_t wd = sw128_desc(src + kWideHalf, 16, 1024);
+        const int slot = i % kWideSlots;
+        if (ok && i >= kWideSlots) ok = mbar_wait(freed + 8 * slot, ((i / kWideSlots) + 1) & 1, kGemmWaitCycles);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int j = 0; j < kFp8Group / 32; ++j)
+          umma_f8_pair(tmem + slot * kWideCols, ad + 2 * j, wd + 2 * j, idesc, j > 0);
+        umma_commit_pair(done + 8 * s);
+      }
+    }
+    if (warp >= 10) {
+      // The scales arrive as rows of groups, and each epilogue thread needs one row: read by
+      // that thread, every group would be 32 cache lines per warp. Copied flat and turned
+      // over in shared memory, it is one conflict-free load.
+      const int t = threadIdx.x - 32 * 10;
+      int c = 0;
+      bool ok = true;
+      for (int tile = pair; tile < tiles && ok; tile += pairs) {
+        const int token0 = (tile % tiles_m) * 256 + rank * 128;
+        const int tn = tile / tiles_m;
+        const int tokens = min(128, a.m - token0);  // may be negative: nothing to read
+        const float* sw0 = a.sw + static_cast<int64_t>(GATE ? tn : 2 * tn) * a.groups;
+        const float* sw1 = GATE ? a.su + static_cast<int64_t>(tn) * a.groups
+                                : a.sw + static_cast<int64_t>(min(2 * tn + 1, (a.n + 127) / 128 - 1)) * a.groups;
+        for (int g0 = 0; g0 < a.groups; g0 += kWideChunk, ++c) {
+          const int n = min(kWideChunk, a.groups - g0);
+          if (c >= 2 && !mbar_wait(used + 8 * (c & 1), ((c >> 1) + 1) & 1, kGemmWaitCycles)) {
+            ok = false;
+            break;
+          }
+          float* dst = scales + (c & 1) * kWideScales;
+          const float* src = a.sa + static_cast<int64_t>(token0) * a.groups + g0;
+          const int g = t % kWideChunk;
+          if (g < n)
+            for (int token = t / kWideChunk; token < tokens; token += 64 / kWideChunk)
+              dst[g * 128 + token] = __ldg(src + static_cast<int64_t>(token) * a.groups + g);
+          if (t < 2 * n) dst[kWideChunk * 128 + t] = __ldg((t & 1 ? sw1 : sw0) + g0 + (t >> 1));
+          mbar_arrive(staged + 8 * (c & 1));
+        }
+      }
+    }
+    __syncwarp();
+    if (warp != 9) cluster_wait_acquire();
+  } else {
+    regs_take<224>();
+    cluster_wait_acquire();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const int part = warp >> 2;
+    const int token_in = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    int i = 0, chunk = 0;
+    bool ok = true;
+    const auto next_chunk = [&] {  // this warp is done with a chunk of scales
+      __syncwarp();
+      if (lane == 0) mbar_arrive(used + 8 * (chunk & 1));
+      ++chunk;
+    };
+    for (int tile = pair, parity = 0; tile < tiles; tile += pairs, parity ^= 1) {
+      const int token = (tile % tiles_m) * 256 + rank * 128 + token_in;
+      const int tn = tile / tiles_m;
+      const bool live = token < a.m;
+      const int blocks = (a.n + 127) / 128;
+      float acc[128];  // GATE: 64 columns of G, then the same of U
+#pragma unroll
+      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+      for (int g = 0; g < a.groups; ++g, ++i) {
+        if (g % kWideChunk == 0) {
+          if (g > 0) next_chunk();
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(staged + 8 * (chunk & 1), (chunk >> 1) & 1, kGemmWaitCycles));
+        }
+        const float* sc = scales + (chunk & 1) * kWideScales + (g % kWideChunk) * 128;
+        const float sa = sc[token_in];
+        const float2 sw = *reinterpret_cast<const float2*>(scales + (chunk & 1) * kWideScales + kWideChunk * 128 +
+                                                           2 * (g % kWideChunk));
+        const float f0 = sa * (GATE || part == 0 ? sw.x : sw.y), f1 = sa * sw.y;
+        const int slot = i % kWideSlots;
+        const int s = i % kWideStages;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(done + 8 * s, (i / kWideStages) & 1, kGemmWaitCycles));
+        if (!ok) continue;
+        tc_fence_after();
+        // the next 32 columns are on their way from TMEM while these are added
+        const uint32_t src = tmem + lanes + slot * kWideCols + part * (GATE ? 64 : 128);
+        uint32_t p[2][32];
+        tmem_ld32(src, p[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_wait_ld();
+          if (c < 3) {
+            tmem_ld32(src + (GATE ? ((c + 1) >> 1) * 128 + ((c + 1) & 1) * 32 : (c + 1) * 32), p[(c + 1) & 1]);
+          } else {  // every column is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(freed + 8 * slot);
+          }
+          const float2 f = GATE && c >= 2 ? make_float2(f1, f1) : make_float2(f0, f0);
+          float2* ac = reinterpret_cast<float2*>(acc + c * 32);
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            ac[j] = fma2(make_float2(__uint_as_float(p[c & 1][2 * j]), __uint_as_float(p[c & 1][2 * j + 1])), f, ac[j]);
+        }
+      }
+      next_chunk();
+      if (!ok) {  // a wait that ran out leaves NaN, not a stale tile
+#pragma unroll
+        for (int j = 0; j < 128; ++j) acc[j] = __int_as_float(0x7fc00000);
+      }
+      if (GATE) {
+        const int col0 = tn * 128 + part * 64;
+        float amax = 0.f;
+#pragma unroll
+        for (int j = 0; j < 64; ++j) {
+          acc[j] = silu_times(acc[j], acc[64 + j]);
+          if (col0 + j < a.n) amax = max_nan(amax, fabsf(acc[j]));
+        }
+        amax_part[parity][part][token_in] = amax;
+        named_bar_sync(1, 256);
+        amax = max_nan(max_nan(amax, amax_part[parity][part ^ 1][token_in]), kFp8Floor);
+        const float inverse = __fdiv_rn(kFp8Max, amax);
+        if (live) {
+          uint8_t* q = static_cast<uint8_t*>(a.out) + static_cast<int64_t>(token) * a.n + col0;
+#pragma unroll
+          for (int j = 0; j < 64; j += 16)  // n is a multiple of 16
+            if (col0 + j < a.n) *reinterpret_cast<uint4*>(q + j) = codes16(acc + j, inverse);
+          if (part == 0) a.out_scale[static_cast<int64_t>(token) * blocks + tn] = __fdiv_rn(amax, kFp8Max);
+        }
+      } else if (live) {
+        const bool vector = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 && (a.n & (a.out_f32 ? 7 : 15)) == 0;
+        const int col0 = tn * 256 + part * 128;
+        const int64_t at = static_cast<int64_t>(token) * a.n + col0;
+        if (a.out_f32)
+          store_columns_f32(static_cast<float*>(a.out) + at, a.n - col0, vector, acc, 128);
+        else
+          store_columns_bf16(static_cast<__nv_bfloat16*>(a.out) + at, a.n - col0, vector, acc, 128);
+      }
+    }
+  }
+  tc_fence_before();
+  cluster_sync_all();  // the other block's copies, arrivals and products are done with this one
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_slot, kWideTmem);
+  }
+}
+
 namespace {
 
 using FnEncode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -344,8 +647,40 @@ cudaError_t launch_gemm(const GemmCall& c, int splits, cudaStream_t stream) {
 }
 
 template <bool GATE>
+cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
+  CUtensorMap wmap, umap, amap;
+  if (!encode_tiles(&wmap, c.w, c.args.n, c.k, c.ws, 128) || !encode_tiles(&amap, c.a, c.args.m, c.k, c.as, 128))
+    return cudaErrorInvalidValue;
+  umap = wmap;
+  if (GATE && !encode_tiles(&umap, c.u, c.args.n, c.k, c.us, 128)) return cudaErrorInvalidValue;
+  const cudaError_t e =
+      cudaFuncSetAttribute(fp8_wide_kernel<GATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+  if (e != cudaSuccess) return e;
+  const int columns = GATE ? 128 : 256;
+  const int64_t tiles = static_cast<int64_t>((c.args.m + 255) / 256) * ((c.args.n + columns - 1) / columns);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * static_cast<unsigned>(tiles < 74 ? tiles : 74));
+  cfg.blockDim = dim3(kWideThreads);
+  cfg.dynamicSmemBytes = kWideSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, fp8_wide_kernel<GATE>, wmap, umap, amap, c.args);
+}
+
+template <bool GATE>
 cudaError_t launch_gemm_rows(const GemmCall& c, cudaStream_t stream) {
   const GemmArgs& a = c.args;
+  const int columns = GATE ? 128 : 256;
+  if (a.m >= 256 && static_cast<int64_t>((a.m + 255) / 256) * ((a.n + columns - 1) / columns) >= 37)
+    return launch_wide<GATE>(c, stream);
   const int nt = a.m <= 16 ? 16 : a.m <= 32 ? 32 : 64;
   const int64_t tiles = static_cast<int64_t>((a.n + kTileRows - 1) / kTileRows) * ((a.m + nt - 1) / nt);
   int splits = 1;  // as many blocks as one wave of the 148 SMs holds, a column group each at least
