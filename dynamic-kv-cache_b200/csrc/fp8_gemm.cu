@@ -29,10 +29,12 @@ namespace dkv {
 using namespace ptx;
 
 constexpr long long kGemmWaitCycles = 400000000LL;  // ~0.2 s: a healthy wait is microseconds
-constexpr int kGemmStages = 4;
+constexpr int kGemmStages = 4;     // operand stages at most
 constexpr int kGemmSlots = 4;      // accumulators in TMEM, one column group each
-constexpr int kGemmThreads = 192;  // warps 0-3: scale and add; 4: copies; 5: MMA issue
+constexpr int kGemmThreads = 256;  // warps 0-3: scale and add; 4: copies; 5: MMA issue; all: the final sums
 constexpr int kTileRows = 128;     // weight rows of a tile
+constexpr int kMaxSplits = 16;
+constexpr int kMaxSmem = 228 * 1024 - 3 * 1536;  // of an SM, without the blocks' static and reserved parts
 
 struct GemmArgs {
   const float* sa;         // [m, groups]
@@ -40,7 +42,7 @@ struct GemmArgs {
   const float* su;         // GATE: the same for the up weights
   void* out;               // [m, n] bf16 / fp32, or e4m3 with GATE
   float* out_scale;        // GATE: [m, ceil(n / 128)]
-  int m, n, groups, splits;
+  int m, n, groups, splits, stages;
   int out_f32;
 };
 
@@ -51,13 +53,17 @@ struct GemmTile {
   static constexpr int kTokenBytes = NT * kFp8Group;
   static constexpr int kStageBytes = kParts * kWeightBytes + kTokenBytes;
   static constexpr int kCols = NT * kParts;  // TMEM columns of one accumulator
-  static constexpr int kTmemCols = kCols * kGemmSlots < 32 ? 32 : kCols * kGemmSlots;
-  static constexpr int kRingBytes = kGemmStages * kStageBytes;
-  static constexpr int kPartialBytes = kParts * NT * kTileRows * 4;  // reuses the ring
-  static_assert(kPartialBytes <= kRingBytes, "partial sums fit the operand ring");
-  static_assert(kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM allocation");
-  static size_t smem(int groups_per_split) {
-    return 1024 + kRingBytes + static_cast<size_t>(kParts) * groups_per_split * NT * 4;
+  static constexpr int kTmemCols = kCols * kGemmSlots;
+  // blocks per SM: while one starts, loads or sums up, others keep the copies going
+  static constexpr int kBlocks = kCols <= 32 ? 3 : 2;
+  static_assert(kParts * NT * kTileRows * 4 <= 2 * kStageBytes, "one block's sums fit the smallest operand ring");
+  static_assert(kTmemCols * kBlocks <= 512 && kTmemCols >= 32 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM allocation");
+  // operand ring, partial sums of `splits` blocks (one block's reuse the ring), scale products
+  static int mail_bytes(int splits) {
+    return splits > 1 ? kParts * splits * ((NT + splits - 1) / splits) * kTileRows * 4 : 0;
+  }
+  static int smem(int stages, int splits, int groups_per_split) {
+    return 1024 + stages * kStageBytes + mail_bytes(splits) + kParts * groups_per_split * NT * 4;
   }
 };
 
@@ -72,19 +78,27 @@ __device__ __forceinline__ float silu_times(float g, float u) {
 }
 
 template <int NT, bool GATE>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(kGemmThreads, GemmTile<NT, GATE>::kBlocks)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap umap,
                 const __grid_constant__ CUtensorMap amap, const GemmArgs a) {
   using T = GemmTile<NT, GATE>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * kGemmStages + 2 * kGemmSlots];
+  __shared__ __align__(8) uint64_t bars[2 * kGemmStages + 2 * kGemmSlots + 1];
   __shared__ uint32_t tmem_slot;
   const uint32_t ring = (smem_addr(smem_raw) + 1023u) & ~1023u;
-  float* scales = reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)) + T::kRingBytes);
+  uint8_t* const ring_ptr = smem_raw + (ring - smem_addr(smem_raw));
+  // this block's own partial sums [part][token][weight row], in the ring once it is read
+  float* const own = reinterpret_cast<float*>(ring_ptr);
+  // ... and every block's for the tokens that it adds up: [rank][part][token][weight row]
+  const int local = (NT + a.splits - 1) / a.splits;
+  const uint32_t mail = ring + a.stages * T::kStageBytes;
+  float* const scales = reinterpret_cast<float*>(
+      ring_ptr + a.stages * T::kStageBytes + (a.splits > 1 ? a.splits * T::kParts * local * kTileRows * 4 : 0));
   const uint32_t full = smem_addr(bars);
   const uint32_t empty = full + 8 * kGemmStages;
   const uint32_t done = empty + 8 * kGemmStages;  // an accumulator is complete
   const uint32_t freed = done + 8 * kGemmSlots;   // ... and read
+  const uint32_t mailed = freed + 8 * kGemmSlots; // the mail is complete
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -94,56 +108,64 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   const int per = (a.groups + a.splits - 1) / a.splits;
   const int group0 = rank * per;
   const int count = max(0, min(per, a.groups - group0));
+  const int live = min(NT, a.m - token0);
+  const int mine = max(0, min(local, live - rank * local));  // tokens that this block adds up
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * kGemmStages + kGemmSlots; ++i) mbar_init(full + 8 * i, 1);
     for (int i = 0; i < kGemmSlots; ++i) mbar_init(freed + 8 * i, 128);
+    mbar_init(mailed, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 4 && lane == 0) {
     prefetch_tensor_map(&wmap);
     if (GATE) prefetch_tensor_map(&umap);
     prefetch_tensor_map(&amap);
+    // The weights of the first stages set out for L2 while the previous kernel finishes.
+    for (int i = 0; i < min(count, a.stages); ++i) {
+      tile2d_prefetch(&wmap, (group0 + i) * kFp8Group, tile * kTileRows);
+      if (GATE) tile2d_prefetch(&umap, (group0 + i) * kFp8Group, tile * kTileRows);
+    }
   }
-  pdl_wait();  // operands are the previous kernels' output
-  // TMEM is taken after the wait and before the trigger: a waiting block never holds what
-  // the grid it waits for still needs, and no dependent starts before every block has it.
-  if (warp == 5) {
-    tmem_alloc(smem_addr(&tmem_slot), T::kTmemCols);
-    tmem_relinquish();
-  }
-  tc_fence_before();
+  if (threadIdx.x == 0 && a.splits > 1) mbar_arrive_expect_tx(mailed, a.splits * T::kParts * mine * kTileRows * 4);
   __syncthreads();
-  tc_fence_after();
-  pdl_trigger();
-  const uint32_t tmem = tmem_slot;
+  if (a.splits > 1) cluster_arrive_release();  // this block has started: others may write to it
+  pdl_wait();  // operands are the previous kernels' output
 
   if (warp == 4) {
     if (lane == 0) {
       int i = 0;
-      for (; i < count; ++i) {
-        const int s = i % kGemmStages;
-        if (i >= kGemmStages && !mbar_wait(empty + 8 * s, ((i / kGemmStages) + 1) & 1, kGemmWaitCycles)) break;
+      for (int s = 0, phase = 1; i < count; ++i) {
+        if (i >= a.stages && !mbar_wait(empty + 8 * s, phase, kGemmWaitCycles)) break;
         const uint32_t dst = ring + s * T::kStageBytes;
         const int x = (group0 + i) * kFp8Group;
         mbar_arrive_expect_tx(full + 8 * s, T::kStageBytes);
         tile2d_g2s(dst, &wmap, x, tile * kTileRows, full + 8 * s);
         if (GATE) tile2d_g2s(dst + T::kWeightBytes, &umap, x, tile * kTileRows, full + 8 * s);
         tile2d_g2s(dst + T::kParts * T::kWeightBytes, &amap, x, token0, full + 8 * s);
+        if (++s == a.stages) s = 0, phase ^= 1;
       }
       // a wait that ran out: the copies in flight still target this block's memory
       if (i < count)
-        for (int j = max(0, i - kGemmStages); j < i; ++j)
-          mbar_wait(full + 8 * (j % kGemmStages), (j / kGemmStages) & 1, kGemmWaitCycles);
+        for (int j = max(0, i - a.stages); j < i; ++j)
+          mbar_wait(full + 8 * (j % a.stages), (j / a.stages) & 1, kGemmWaitCycles);
     }
     __syncwarp();
   } else if (warp == 5) {
+    // TMEM is taken after the wait and before the trigger: a waiting block never holds what
+    // the grid it waits for still needs, and no dependent starts before every block has it.
+    tmem_alloc(smem_addr(&tmem_slot), T::kTmemCols);
+    tmem_relinquish();
+    pdl_trigger();
+    tc_fence_before();
+    named_bar_arrive(2, 160);  // the products need not wait for the scales
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_e4m3(kTileRows, NT);
-      for (int i = 0; i < count; ++i) {
-        const int s = i % kGemmStages;
+      for (int i = 0, s = 0, phase = 0; i < count; ++i) {
         const int slot = i % kGemmSlots;
-        bool ok = mbar_wait(full + 8 * s, (i / kGemmStages) & 1, kGemmWaitCycles);
+        bool ok = mbar_wait(full + 8 * s, phase, kGemmWaitCycles);
         if (ok && i >= kGemmSlots) ok = mbar_wait(freed + 8 * slot, ((i / kGemmSlots) + 1) & 1, kGemmWaitCycles);
         if (!ok) break;
         tc_fence_after();
@@ -156,12 +178,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
           umma_f8(tmem + slot * T::kCols, wd + 2 * j, ad + 2 * j, idesc, j > 0);
           if (GATE) umma_f8(tmem + slot * T::kCols + NT, ud + 2 * j, ad + 2 * j, idesc, j > 0);
         }
-        umma_commit(empty + 8 * s);
         umma_commit(done + 8 * slot);
+        umma_commit(empty + 8 * s);
+        if (++s == a.stages) s = 0, phase ^= 1;
       }
     }
     __syncwarp();
-  } else {
+  } else if (warp < 4) {
     // the scale products of this block's groups: scales[part][group][token]
     for (int i = threadIdx.x; i < count * NT; i += 128) {
       const int token = i / count;
@@ -171,7 +194,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       scales[g * NT + token] = s * a.sw[block];
       if (GATE) scales[(count + g) * NT + token] = s * a.su[block];
     }
-    named_bar_sync(1, 128);
+    tc_fence_before();
+    named_bar_sync(2, 160);  // the scales of all four warps, and TMEM's address
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    constexpr int kStep = T::kCols <= 32 ? 16 : 32;
     float acc[T::kCols];
 #pragma unroll
     for (int j = 0; j < T::kCols; ++j) acc[j] = 0.f;
@@ -183,58 +210,81 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < T::kCols; c += 16) {
-        uint32_t p[16];
-        tmem_ld16(tmem + lanes + slot * T::kCols + c, p);
+      for (int c = 0; c < T::kCols; c += kStep) {
+        uint32_t p[kStep];
+        if constexpr (kStep == 32) {
+          tmem_ld32(tmem + lanes + slot * T::kCols + c, p);
+        } else {
+          tmem_ld16(tmem + lanes + slot * T::kCols + c, p);
+        }
         tmem_wait_ld();
         const float* sc = scales + (c < NT ? i * NT + c : (count + i) * NT + c - NT);
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
+        for (int j = 0; j < kStep; j += 4) {
           const float4 f = *reinterpret_cast<const float4*>(sc + j);
-          acc[c + j] = fmaf(__uint_as_float(p[j]), f.x, acc[c + j]);
-          acc[c + j + 1] = fmaf(__uint_as_float(p[j + 1]), f.y, acc[c + j + 1]);
-          acc[c + j + 2] = fmaf(__uint_as_float(p[j + 2]), f.z, acc[c + j + 2]);
-          acc[c + j + 3] = fmaf(__uint_as_float(p[j + 3]), f.w, acc[c + j + 3]);
+          float2* ac = reinterpret_cast<float2*>(acc + c + j);
+          ac[0] = fma2(make_float2(__uint_as_float(p[j]), __uint_as_float(p[j + 1])), make_float2(f.x, f.y), ac[0]);
+          ac[1] = fma2(make_float2(__uint_as_float(p[j + 2]), __uint_as_float(p[j + 3])), make_float2(f.z, f.w), ac[1]);
         }
       }
       tc_fence_before();
       mbar_arrive(freed + 8 * slot);
     }
-    // partial sums [part][token][weight row]; a wait that ran out leaves NaN, not a stale tile
-    float* partial = reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)));
+    // a wait that ran out leaves NaN, not a stale tile
 #pragma unroll
-    for (int j = 0; j < T::kCols; ++j) partial[j * kTileRows + threadIdx.x] = ok ? acc[j] : __int_as_float(0x7fc00000);
+    for (int j = 0; j < T::kCols; ++j) own[j * kTileRows + threadIdx.x] = ok ? acc[j] : __int_as_float(0x7fc00000);
+    if (a.splits > 1) {
+      // Rank r adds up tokens [r * local, (r + 1) * local): one bulk copy per rank and part
+      // (single stores to another block's shared memory were 5 times slower).
+      fence_proxy_async_smem();
+      cluster_wait_acquire();
+      named_bar_sync(3, 128);
+      const int to = threadIdx.x;
+      const int n = min(local, live - to * local);
+      if (to < a.splits && n > 0) {
+#pragma unroll
+        for (int p = 0; p < T::kParts; ++p)
+          bulk_s2s(dsmem_addr(mail + (rank * T::kParts + p) * local * kTileRows * 4, to),
+                   ring + (p * NT + to * local) * kTileRows * 4, n * kTileRows * 4, dsmem_addr(mailed, to));
+      }
+    }
   }
+  if (a.splits > 1 && warp >= 4) cluster_wait_acquire();
   // TMEM goes back before this block waits for another one: what holds TMEM never depends
   // on a block that may still be waiting for some.
   tc_fence_before();
   __syncthreads();
   if (warp == 5) {
     tc_fence_after();
-    tmem_dealloc(tmem, T::kTmemCols);
+    tmem_dealloc(tmem_slot, T::kTmemCols);
   }
-  if (a.splits > 1) cluster_sync_all();
+  const float* sums = own;
+  int parts_apart = NT * kTileRows;
+  bool complete = true;
+  if (a.splits > 1) {
+    sums = reinterpret_cast<const float*>(ring_ptr + a.stages * T::kStageBytes);
+    parts_apart = local * kTileRows;
+    if (mine > 0) complete = mbar_wait(mailed, 0, kGemmWaitCycles);
+  }
 
   // a warp per token, 4 weight rows (output columns) per lane
   const int col = tile * kTileRows + lane * 4;
-  for (int t = rank + a.splits * warp; t < NT && token0 + t < a.m; t += a.splits * (kGemmThreads / 32)) {
+  const int first = a.splits > 1 ? rank * local : 0;
+  for (int i = warp; i < (a.splits > 1 ? mine : live); i += kGemmThreads / 32) {
+    const int t = first + i;
     float4 sum[T::kParts];
 #pragma unroll
     for (int p = 0; p < T::kParts; ++p) {
-      const uint32_t at = ring + ((p * NT + t) * kTileRows + lane * 4) * 4;
-      sum[p] = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int r = 0; r < a.splits; ++r) {
-        float4 v;
-        if (a.splits > 1) {
-          v = ld_dsmem_f4(dsmem_addr(at, r));
-        } else {
-          v = *reinterpret_cast<const float4*>(smem_raw + (at - smem_addr(smem_raw)));
-        }
+      const float* at = sums + p * parts_apart + i * kTileRows + lane * 4;
+      sum[p] = *reinterpret_cast<const float4*>(at);
+      for (int r = 1; r < a.splits; ++r) {
+        const float4 v = *reinterpret_cast<const float4*>(at + r * T::kParts * parts_apart);
         sum[p].x += v.x;
         sum[p].y += v.y;
         sum[p].z += v.z;
         sum[p].w += v.w;
       }
+      if (!complete) sum[p].x = sum[p].y = sum[p].z = sum[p].w = __int_as_float(0x7fc00000);
     }
     const int64_t row = token0 + t;
     if (GATE) {  // n is a multiple of 16: a lane's 4 columns are all inside or all outside
@@ -278,7 +328,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       }
     }
   }
-  if (a.splits > 1) cluster_sync_all();  // the other blocks may still be reading this one's partial sums
+  if (a.splits > 1) {  // the copies out of this block's memory have arrived; nothing to order:
+    cluster_arrive_relaxed();  // a release would wait for this block's stores first
+    cluster_wait_acquire();
+  }
 }
 
 // ---- many tokens -----------------------------------------------------------------
@@ -294,41 +347,61 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
 // GATE makes the halves the gate and the up rows of the same 128 intermediate columns:
 // each thread then holds matching columns of G and U.
 constexpr int kWideThreads = 384;  // warps 0-7: scale and add; 8: copies; 9: MMA issue; 10, 11: none
-constexpr int kWideStages = 6;
+constexpr int kWideStages = 5;
 constexpr int kWideHalf = 128 * kFp8Group;  // bytes of one block's operand tile of one group
 constexpr int kWideStageBytes = 2 * kWideHalf;
 constexpr int kWideChunk = 16;  // groups whose scales are staged at a time
 constexpr int kWideScales = kWideChunk * 128 + 2 * kWideChunk;  // [group][token], then [group][half] of the weights
-constexpr int kWideSmem = 1024 + kWideStages * kWideStageBytes + 2 * kWideScales * 4;
+constexpr int kWideSmem = 1024 + kWideStages * kWideStageBytes + 2 * kWideScales * 4 + 8 * 32 * 128;
 constexpr int kWideCols = 256;
 constexpr int kWideSlots = 2;
 constexpr uint32_t kWideTmem = kWideSlots * kWideCols;
 
-// `count` columns of one token (a multiple of 16), of which `columns` exist.
-__device__ __forceinline__ void store_columns_bf16(__nv_bfloat16* p, int columns, bool vector, const float* v, int count) {
-  if (vector && columns >= count) {
+// A warp's tile leaves through its piece of shared memory: 32 tokens (one per lane) x 128 bytes,
+// written a row per lane and read back 8 lanes to a row, so that every store instruction fills
+// whole 128-byte lines (a row per lane would touch 32 of them, 16 or 32 bytes each). The
+// 16-byte pieces of row r are exchanged by r % 8: both directions are free of bank conflicts.
+constexpr int kTurnBytes = 32 * 128;
+
+__device__ __forceinline__ uint32_t turn_at(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+
+// Writes `BYTES` (64 or 128) per token, as 16-byte words w, to row `token` (a row is `stride`
+// bytes) from byte `at` on, up to the row's end; rows from `tokens` on are left alone.
+// Rows that do not start on 16 bytes are stored element by element (SIZE bytes each).
+template <int BYTES, int SIZE>
+__device__ __forceinline__ void store_turned(uint8_t* out, int token, int tokens, int64_t stride, int64_t at,
+                                             const uint4* w, uint8_t* turn) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kPieces = BYTES / 16;
+  __syncwarp();  // the last call's reads
 #pragma unroll
-    for (int j = 0; j < count; j += 16) {
-      float w[8];
+  for (int c = 0; c < kPieces; ++c) *reinterpret_cast<uint4*>(turn + turn_at(lane, c)) = w[c];
+  __syncwarp();
+  const int first = token - lane;
+  if (stride % 16 == 0) {
+    const int c = lane % kPieces;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = __uint_as_float(pack_bf16x2(v[j + 2 * i], v[j + 2 * i + 1]));
-      st_global_v8(reinterpret_cast<float*>(p + j), w);
+    for (int r = lane / kPieces; r < 32; r += 32 / kPieces) {
+      if (first + r < tokens && at + c * 16 < stride)
+        *reinterpret_cast<uint4*>(out + (first + r) * stride + at + c * 16) =
+            *reinterpret_cast<const uint4*>(turn + turn_at(r, c));
     }
   } else {
+#pragma unroll 4
+    for (int r = 0; r < 32; ++r) {
+      if (first + r >= tokens) break;
 #pragma unroll
-    for (int j = 0; j < count; ++j)
-      if (j < columns) p[j] = __float2bfloat16_rn(v[j]);
-  }
-}
-
-__device__ __forceinline__ void store_columns_f32(float* p, int columns, bool vector, const float* v, int count) {
-  if (vector && columns >= count) {
-#pragma unroll
-    for (int j = 0; j < count; j += 8) st_global_v8(p + j, v + j);
-  } else {
-#pragma unroll
-    for (int j = 0; j < count; ++j)
-      if (j < columns) p[j] = v[j];
+      for (int b = lane * SIZE; b < BYTES; b += 32 * SIZE) {
+        const uint8_t* src = turn + turn_at(r, b >> 4) + (b & 15);
+        uint8_t* dst = out + (first + r) * stride + at + b;
+        if (at + b >= stride) break;
+        if constexpr (SIZE == 4) {
+          *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+        } else {
+          *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
+        }
+      }
+    }
   }
 }
 
@@ -482,6 +555,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     const int part = warp >> 2;
     const int token_in = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    uint8_t* const turn = reinterpret_cast<uint8_t*>(scales + 2 * kWideScales) + warp * kTurnBytes;
     int i = 0, chunk = 0;
     bool ok = true;
     const auto next_chunk = [&] {  // this warp is done with a chunk of scales
@@ -541,30 +615,44 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       if (GATE) {
         const int col0 = tn * 128 + part * 64;
         float amax = 0.f;
+        const int inside = a.n - col0;  // a multiple of 16, like the columns below
 #pragma unroll
-        for (int j = 0; j < 64; ++j) {
-          acc[j] = silu_times(acc[j], acc[64 + j]);
-          if (col0 + j < a.n) amax = max_nan(amax, fabsf(acc[j]));
+        for (int j = 0; j < 64; j += 16) {
+          float m = 0.f;
+#pragma unroll
+          for (int i = j; i < j + 16; ++i) {
+            acc[i] = silu_times(acc[i], acc[64 + i]);
+            m = max_nan(m, fabsf(acc[i]));
+          }
+          if (j < inside) amax = max_nan(amax, m);
         }
         amax_part[parity][part][token_in] = amax;
         named_bar_sync(1, 256);
         amax = max_nan(max_nan(amax, amax_part[parity][part ^ 1][token_in]), kFp8Floor);
         const float inverse = __fdiv_rn(kFp8Max, amax);
-        if (live) {
-          uint8_t* q = static_cast<uint8_t*>(a.out) + static_cast<int64_t>(token) * a.n + col0;
+        uint4 w[4];
 #pragma unroll
-          for (int j = 0; j < 64; j += 16)  // n is a multiple of 16
-            if (col0 + j < a.n) *reinterpret_cast<uint4*>(q + j) = codes16(acc + j, inverse);
-          if (part == 0) a.out_scale[static_cast<int64_t>(token) * blocks + tn] = __fdiv_rn(amax, kFp8Max);
+        for (int j = 0; j < 4; ++j) w[j] = codes16(acc + 16 * j, inverse);
+        store_turned<64, 1>(static_cast<uint8_t*>(a.out), token, a.m, a.n, col0, w, turn);  // n is a multiple of 16
+        if (live && part == 0) a.out_scale[static_cast<int64_t>(token) * blocks + tn] = __fdiv_rn(amax, kFp8Max);
+      } else if (a.out_f32) {
+#pragma unroll
+        for (int j = 0; j < 128; j += 32)
+          store_turned<128, 4>(static_cast<uint8_t*>(a.out), token, a.m, 4LL * a.n, 4LL * (tn * 256 + part * 128 + j),
+                               reinterpret_cast<const uint4*>(acc + j), turn);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 128; j += 64) {
+          uint4 w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float* v = acc + j + 8 * i;
+            w[i] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                              pack_bf16x2(v[6], v[7]));
+          }
+          store_turned<128, 2>(static_cast<uint8_t*>(a.out), token, a.m, 2LL * a.n, 2LL * (tn * 256 + part * 128 + j), w,
+                               turn);
         }
-      } else if (live) {
-        const bool vector = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 && (a.n & (a.out_f32 ? 7 : 15)) == 0;
-        const int col0 = tn * 256 + part * 128;
-        const int64_t at = static_cast<int64_t>(token) * a.n + col0;
-        if (a.out_f32)
-          store_columns_f32(static_cast<float*>(a.out) + at, a.n - col0, vector, acc, 128);
-        else
-          store_columns_bf16(static_cast<__nv_bfloat16*>(a.out) + at, a.n - col0, vector, acc, 128);
       }
     }
   }
@@ -625,9 +713,13 @@ cudaError_t launch_gemm(const GemmCall& c, int splits, cudaStream_t stream) {
   if (GATE && !encode_tiles(&umap, c.u, c.args.n, c.k, c.us, kTileRows)) return cudaErrorInvalidValue;
   GemmArgs args = c.args;
   args.splits = splits;
-  const size_t smem = T::smem((args.groups + splits - 1) / splits);
-  const cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<NT, GATE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(smem));
+  const int per = (args.groups + splits - 1) / splits;
+  args.stages = per < 2 ? 2 : per < kGemmStages ? per : kGemmStages;
+  while (args.stages > 2 && T::smem(args.stages, splits, per) > kMaxSmem / T::kBlocks) --args.stages;
+  const int smem = T::smem(args.stages, splits, per);
+  cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<NT, GATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && splits > 8)
+    e = cudaFuncSetAttribute(fp8_gemm_kernel<NT, GATE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((args.n + kTileRows - 1) / kTileRows * splits, (args.m + NT - 1) / NT);
@@ -675,20 +767,64 @@ cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, fp8_wide_kernel<GATE>, wmap, umap, amap, c.args);
 }
 
+// Which kernel, how many tokens per tile and how many blocks per tile: the least time by a
+// model fitted to a sweep of all of them over 34 shapes (1 to 8192 tokens, 128 to 49280
+// weight rows, 256 to 16384 columns; inputs beyond L2; us on a B200, the model within ~15 %):
+//   split kernel  2.4 + stream + sums, where one wave of blocks streams its operands at 62
+//                 bytes/ns per SM, and r waves take r * (0.9 + bytes / 85); the partial sums
+//                 of a split tile cross between SMs at 0.023 per token column
+//   pair kernel   4.2 + per wave of 74 tiles: 0.44 per column group + 1.7 (GATE: 2.2) per tile
+// Measured either side of its borders: 512 x 960 x 960 5.5 us by 32 tokens (64: 6.1, pairs
+// 9.5); 64 x 960 x 2560 4.4 by 32 tokens and 5 blocks a tile (one: 9.3); 2048 x 1600 x 960
+// 10.0 by pairs (64 tokens: 12.8).
+struct GemmPlan {
+  int tokens;  // per tile; 256: the pair kernel
+  int splits;
+};
+
+GemmPlan make_gemm_plan(int m, int n, int groups, bool gate) {
+  const int parts = gate ? 2 : 1;
+  const int wide_columns = gate ? 128 : 256;
+  const int64_t wide_tiles = static_cast<int64_t>((m + 255) / 256) * ((n + wide_columns - 1) / wide_columns);
+  GemmPlan best{256, 1};
+  float least = 4.2f + static_cast<float>((wide_tiles + 73) / 74) * (groups * 0.44f + (gate ? 2.2f : 1.7f));
+  for (int nt = 16; nt <= (gate ? 32 : 64); nt *= 2) {
+    const int64_t tiles = static_cast<int64_t>((n + kTileRows - 1) / kTileRows) * ((m + nt - 1) / nt);
+    if (tiles > INT32_MAX / kMaxSplits || (m + nt - 1) / nt > 65535) continue;
+    const float stage = (parts * kTileRows + nt) * kFp8Group * 1e-3f;
+    for (int s = 1; s <= kMaxSplits && s <= groups; ++s) {
+      const int per = (groups + s - 1) / s;
+      if ((groups + per - 1) / per != s) continue;  // a block would have nothing to do
+      const int64_t blocks = tiles * s;
+      // blocks that start at once, one per SM: clusters stay within a GPC, of which there are
+      // eight of at least 16 SMs, and sizes that do not divide 16 pack less tightly
+      const float room = s == 1 ? 148.f : 16 % s == 0 ? 128.f : 0.9f * 8 * (18 / s) * s;
+      float time = 2.4f + (s > 1 ? 0.023f * nt * parts : 0.f);
+      if (blocks <= room) {
+        time += per * stage / 62.f;
+      } else {
+        float waves = 2.f;  // two blocks share an SM
+        if (blocks > 2 * room) waves = s == 1 ? blocks / 148.f : 2.f * static_cast<int>((blocks + 2 * room - 1) / (2 * room));
+        time += waves * (0.9f + per * stage / 85.f);
+      }
+      if (time < least) {
+        least = time;
+        best = {nt, s};
+      }
+      if (blocks > 4 * 148) break;  // more blocks only add their own start
+    }
+  }
+  return best;
+}
+
 template <bool GATE>
-cudaError_t launch_gemm_rows(const GemmCall& c, cudaStream_t stream) {
-  const GemmArgs& a = c.args;
-  const int columns = GATE ? 128 : 256;
-  if (a.m >= 256 && static_cast<int64_t>((a.m + 255) / 256) * ((a.n + columns - 1) / columns) >= 37)
-    return launch_wide<GATE>(c, stream);
-  const int nt = a.m <= 16 ? 16 : a.m <= 32 ? 32 : 64;
-  const int64_t tiles = static_cast<int64_t>((a.n + kTileRows - 1) / kTileRows) * ((a.m + nt - 1) / nt);
-  int splits = 1;  // as many blocks as one wave of the 148 SMs holds, a column group each at least
-  while (splits < 8 && tiles * splits * 2 <= 148 && splits * 2 <= a.groups) splits *= 2;
-  switch (nt) {
-    case 16: return launch_gemm<16, GATE>(c, splits, stream);
-    case 32: return launch_gemm<32, GATE>(c, splits, stream);
-    default: return launch_gemm<64, GATE>(c, splits, stream);
+cudaError_t launch_planned(const GemmCall& c, cudaStream_t stream) {
+  const GemmPlan p = make_gemm_plan(c.args.m, c.args.n, c.args.groups, GATE);
+  switch (p.tokens) {
+    case 16: return launch_gemm<16, GATE>(c, p.splits, stream);
+    case 32: return launch_gemm<32, GATE>(c, p.splits, stream);
+    case 64: return launch_gemm<GATE ? 32 : 64, GATE>(c, p.splits, stream);
+    default: return launch_wide<GATE>(c, stream);
   }
 }
 
@@ -697,7 +833,7 @@ cudaError_t launch_gemm_rows(const GemmCall& c, cudaStream_t stream) {
 cudaError_t launch_fp8_linear(const void* a, const float* sa, const void* w, const float* sw, void* out, int out_f32,
                               int m, int n, int k, int64_t as, int64_t ws, cudaStream_t stream) {
   const int groups = (k + kFp8Group - 1) / kFp8Group;
-  return launch_gemm_rows<false>({a, w, nullptr, as, ws, 0, k, {sa, sw, nullptr, out, nullptr, m, n, groups, 1, out_f32}},
+  return launch_planned<false>({a, w, nullptr, as, ws, 0, k, {sa, sw, nullptr, out, nullptr, m, n, groups, 1, 0, out_f32}},
                                  stream);
 }
 
@@ -705,7 +841,7 @@ cudaError_t launch_fp8_gate_up(const void* a, const float* sa, const void* gate,
                                const float* su, void* out, float* out_scale, int m, int n, int k, int64_t as,
                                int64_t gs, int64_t us, cudaStream_t stream) {
   const int groups = (k + kFp8Group - 1) / kFp8Group;
-  return launch_gemm_rows<true>({a, gate, up, as, gs, us, k, {sa, sg, su, out, out_scale, m, n, groups, 1, 0}}, stream);
+  return launch_planned<true>({a, gate, up, as, gs, us, k, {sa, sg, su, out, out_scale, m, n, groups, 1, 0, 0}}, stream);
 }
 
 }  // namespace dkv

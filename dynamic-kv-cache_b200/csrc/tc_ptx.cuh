@@ -106,7 +106,14 @@ __device__ __forceinline__ void tile2d_g2s(uint32_t dst, const void* map, int x,
       : "memory");
 }
 
-// The same from a block of a CTA pair: `bar` may lie in the other block (dsmem_addr).
+// Brings a tile into L2 only: no shared memory, no completion, and safe before pdl_wait, since a
+// later write by the previous grid still meets the line in L2.
+__device__ __forceinline__ void tile2d_prefetch(const void* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n" ::"l"(map), "r"(x), "r"(y)
+               : "memory");
+}
+
+// tile2d_g2s from a block of a CTA pair: `bar` may lie in the other block (dsmem_addr).
 __device__ __forceinline__ void tile2d_g2s_pair(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
@@ -129,6 +136,11 @@ __device__ __forceinline__ void regs_give() { asm volatile("setmaxnreg.dec.sync.
 // Barrier among `count` threads (a multiple of 32) using hardware barrier `id` (1..15).
 __device__ __forceinline__ void named_bar_sync(int id, int count) {
   asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(count) : "memory");
+}
+
+// Counts this warp in at a hardware barrier that others wait on.
+__device__ __forceinline__ void named_bar_arrive(int id, int count) {
+  asm volatile("bar.arrive %0, %1;\n" ::"r"(id), "r"(count) : "memory");
 }
 
 __device__ __forceinline__ void fence_proxy_async_smem() {
@@ -331,6 +343,15 @@ __device__ __forceinline__ float2 ld_dsmem_f2(uint32_t addr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
+}
+
+// Bulk copy from this block's shared memory to another's, completing in bytes on an mbarrier
+// there (16-byte aligned, a multiple of 16 bytes; generic writes of the source are fenced first).
+__device__ __forceinline__ void bulk_s2s(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst),
+      "r"(src), "r"(bytes), "r"(bar)
+      : "memory");
 }
 
 // Shared-memory matrix descriptor (sm_100 format) for a 128-byte-swizzled
