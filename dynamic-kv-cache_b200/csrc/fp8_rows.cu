@@ -98,72 +98,110 @@ quantize_weight_kernel(const uint16_t* __restrict__ w, uint8_t* __restrict__ q, 
   if (threadIdx.x == 0) scale[blockIdx.x] = __fdiv_rn(amax, kFp8Max);
 }
 
-// One row per WARPS warps, two chunks of 16 columns per thread: width <= 1024 * WARPS.
-// Rows of one warp share a block of four. The sum of squares runs in fp32 in a fixed order
-// (a thread's columns, a butterfly over the warp, the warps in turn).
+// One row per WARPS warps at a time, two chunks of 16 columns per thread: width <= 1024 *
+// WARPS. Rows of one warp share a block of four. A block works through rows a grid apart: its
+// weights stay in registers, and the next row is on its way while this one is summed up, scaled
+// and stored (one row per block left the memory idle in between: 4097 x 4096 at 3.4 TB/s). A row
+// is held as the bf16 it is (the residual sum is bf16 by definition), half the registers of
+// fp32. The sum of squares runs in fp32 in a fixed order (a thread's columns, a butterfly over
+// the warp, the warps in turn).
 constexpr int kNormFp8Chunks = 2;
+// Blocks per SM: 16 warps (20 without a residual, which needs fewer registers).
 template <int WARPS, bool ADD>
-__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS, 1)
+constexpr int kNormFp8Blocks = WARPS == 1 ? (ADD ? 4 : 5) : WARPS == 16 ? 1 : (ADD ? 16 : 20) / WARPS;
+
+struct NormRow {
+  uint4 x[kNormFp8Chunks][2], y[kNormFp8Chunks][2];
+};
+
+template <int WARPS, bool ADD>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS, kNormFp8Blocks<WARPS, ADD>)
 add_rms_norm_fp8_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ y, uint16_t* __restrict__ x_out,
                         uint8_t* __restrict__ q, float* __restrict__ scale, const uint16_t* __restrict__ weight,
                         int64_t rows, int width, int groups, int64_t xs, int64_t ys, int64_t os, float eps) {
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  const int64_t row = WARPS == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  int64_t row = WARPS == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t step = WARPS == 1 ? static_cast<int64_t>(gridDim.x) * 4 : gridDim.x;
   const int lane = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
-  if (row >= rows) return;  // whole warps leave together, and blocks of more warps have a row
-  float v[kNormFp8Chunks][16];
-  uint4 wv[kNormFp8Chunks][2];  // the weights, loaded with the row (no second round trip)
-  float ss = 0.f;
+  __shared__ float part[2][WARPS];
+  const auto load = [&](int64_t r, NormRow& v) {
+#pragma unroll
+    for (int i = 0; i < kNormFp8Chunks; ++i) {
+      const int c = (lane + 32 * WARPS * i) * 16;
+      if (c >= width || r >= rows) continue;
+      const uint4* a = reinterpret_cast<const uint4*>(x + r * xs + c);
+      v.x[i][0] = a[0];
+      v.x[i][1] = a[1];
+      if (ADD) {
+        const uint4* b = reinterpret_cast<const uint4*>(y + r * ys + c);
+        v.y[i][0] = b[0];
+        v.y[i][1] = b[1];
+      }
+    }
+  };
+  uint4 wv[kNormFp8Chunks][2];
+  NormRow v;
 #pragma unroll
   for (int i = 0; i < kNormFp8Chunks; ++i) {
     const int c = (lane + 32 * WARPS * i) * 16;
-    if (c < width) {
+    wv[i][0] = wv[i][1] = v.x[i][0] = v.x[i][1] = v.y[i][0] = v.y[i][1] = make_uint4(0, 0, 0, 0);
+    if (c < width) {  // columns past the row stay zeros: they add nothing to the sum or the maximum
       wv[i][0] = __ldg(reinterpret_cast<const uint4*>(weight + c));
       wv[i][1] = __ldg(reinterpret_cast<const uint4*>(weight + c) + 1);
-      load16(x + row * xs + c, v[i]);
+    }
+  }
+  load(row, v);
+  for (int turn = 0; row < rows; row += step, turn ^= 1) {  // whole warps, and blocks of more, leave together
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < kNormFp8Chunks; ++i) {
+      float f[16];
+      unpack16(v.x[i][0], v.x[i][1], f);
       if (ADD) {
+        const int c = (lane + 32 * WARPS * i) * 16;
         float b[16];
-        load16(y + row * ys + c, b);
+        unpack16(v.y[i][0], v.y[i][1], b);
         uint32_t s[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = pack_bf16x2(__fadd_rn(v[i][2 * j], b[2 * j]), __fadd_rn(v[i][2 * j + 1], b[2 * j + 1]));
-        uint4* dst = reinterpret_cast<uint4*>(x_out + row * os + c);
-        dst[0] = make_uint4(s[0], s[1], s[2], s[3]);
-        dst[1] = make_uint4(s[4], s[5], s[6], s[7]);
-        unpack16(make_uint4(s[0], s[1], s[2], s[3]), make_uint4(s[4], s[5], s[6], s[7]), v[i]);
+        for (int j = 0; j < 8; ++j) s[j] = pack_bf16x2(__fadd_rn(f[2 * j], b[2 * j]), __fadd_rn(f[2 * j + 1], b[2 * j + 1]));
+        v.x[i][0] = make_uint4(s[0], s[1], s[2], s[3]);
+        v.x[i][1] = make_uint4(s[4], s[5], s[6], s[7]);
+        if (c < width) {
+          uint4* dst = reinterpret_cast<uint4*>(x_out + row * os + c);
+          dst[0] = v.x[i][0];
+          dst[1] = v.x[i][1];
+        }
+        unpack16(v.x[i][0], v.x[i][1], f);
       }
 #pragma unroll
-      for (int j = 0; j < 16; ++j) ss = __fmaf_rn(v[i][j], v[i][j], ss);
+      for (int j = 0; j < 16; ++j) ss = __fmaf_rn(f[j], f[j], ss);
     }
-  }
+    const uint4 now[kNormFp8Chunks][2] = {{v.x[0][0], v.x[0][1]}, {v.x[1][0], v.x[1][1]}};
+    load(row + step, v);
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-  if (WARPS > 1) {
-    __shared__ float part[WARPS];
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = ss;
-    __syncthreads();
-    ss = part[0];
+    for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+    if (WARPS > 1) {  // two sets of partial sums: a warp may be a row ahead of the slowest
+      if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = ss;
+      __syncthreads();
+      ss = part[turn][0];
 #pragma unroll
-    for (int i = 1; i < WARPS; ++i) ss += part[i];
-  }
-  const float rstd = rsqrtf(__fdiv_rn(ss, static_cast<float>(width)) + eps);
+      for (int i = 1; i < WARPS; ++i) ss += part[turn][i];
+    }
+    const float rstd = rsqrtf(__fdiv_rn(ss, static_cast<float>(width)) + eps);
 #pragma unroll
-  for (int i = 0; i < kNormFp8Chunks; ++i) {
-    const int c = (lane + 32 * WARPS * i) * 16;
-    if (32 * WARPS * i * 16 >= width) break;  // the same for every lane
-    float w[16];
-    if (c < width) {
+    for (int i = 0; i < kNormFp8Chunks; ++i) {
+      const int c = (lane + 32 * WARPS * i) * 16;
+      if (32 * WARPS * i * 16 >= width) break;  // the same for every lane
+      float h[16], w[16];
+      unpack16(now[i][0], now[i][1], h);
       unpack16(wv[i][0], wv[i][1], w);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[i][j] = __fmul_rn(__fmul_rn(v[i][j], rstd), w[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[i][j] = 0.f;
+      for (int j = 0; j < 16; ++j) h[j] = __fmul_rn(__fmul_rn(h[j], rstd), w[j]);
+      const float amax = group_max(amax16(h));
+      store_group(h, amax, c < width, c < width && (lane & 7) == 0, q + row * width + c,
+                  scale + row * groups + c / kFp8Group);
     }
-    const float amax = group_max(amax16(v[i]));
-    store_group(v[i], amax, c < width, c < width && (lane & 7) == 0, q + row * width + c,
-                scale + row * groups + c / kFp8Group);
   }
 }
 
@@ -199,7 +237,9 @@ struct NormArgs {
 
 template <int WARPS, bool ADD>
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t stream) {
-  const unsigned blocks = static_cast<unsigned>(WARPS == 1 ? (a.rows + 3) / 4 : a.rows);
+  const int64_t all = WARPS == 1 ? (a.rows + 3) / 4 : a.rows;
+  const int64_t wave = 148 * kNormFp8Blocks<WARPS, ADD>;
+  const unsigned blocks = static_cast<unsigned>(all < wave ? all : wave);
   return launch_rows(blocks, WARPS == 1 ? 128 : 32 * WARPS, stream, add_rms_norm_fp8_kernel<WARPS, ADD>, a.x, a.y,
                      a.x_out, a.q, a.scale, a.weight, a.rows, a.width, a.groups, a.xs, a.ys, a.os, a.eps);
 }
