@@ -9,6 +9,11 @@ bf16. Projections use the joined QKV and gate/up weights of the reference's fuse
 mode (src/gpu_ops.py:26-47). With a GPUCache the attention is the packed-KV path
 (append + attend on the sm_100a kernels); with a NativeCache it is plain bf16
 history + SDPA (the reference's "native" mode).
+
+projections='fp8' (CUDA; not in the reference) runs the projections in 8 bits: the
+joined weights are e4m3 blocks (half the bytes a step has to stream), the norms write
+the e4m3 rows the projections read, and gate, up, SiLU and their product are one
+launch. Residual stream, attention, norms' sums, embeddings and logits stay as they are.
 """
 from dataclasses import dataclass
 
@@ -17,7 +22,10 @@ import torch.nn.functional as F
 
 from . import gpu_kernels as K
 from .gpu_cache import GPUCache, RequestBatch, append_many, attend_many
-from .gpu_ops import activation_product, add_rms, cuda_rms
+from .gpu_ops import (Fp8, activation_product, add_rms, add_rms_fp8, cuda_rms, fp8_gate_up, fp8_linear, fp8_quantize,
+                      fp8_quantize_weight)
+
+PROJECTIONS = ('bf16', 'fp8')
 
 
 @dataclass(frozen=True)
@@ -74,22 +82,54 @@ def apply_rope(x, cos, sin):
     return (xf * cos + rot * sin).to(x.dtype)
 
 
-class Decoder(torch.nn.Module):
-    def __init__(self, cfg=SMOLLM2_360M, device='cuda', dtype=torch.bfloat16, seed=0):
+class Fp8Weight(torch.nn.Module):
+    """8-bit blocks of one bf16 weight [n, k], as buffers."""
+
+    def __init__(self, w):
         super().__init__()
+        q, scale = fp8_quantize_weight(w)
+        self.register_buffer('q', q)
+        self.register_buffer('scale', scale)
+
+    @property
+    def blocks(self):
+        return Fp8(self.q, self.scale)
+
+
+class Decoder(torch.nn.Module):
+    def __init__(self, cfg=SMOLLM2_360M, device='cuda', dtype=torch.bfloat16, seed=0, projections='bf16'):
+        super().__init__()
+        if projections not in PROJECTIONS:
+            raise ValueError(f'projections must be one of {PROJECTIONS}')
+        if projections == 'fp8' and (torch.device(device).type != 'cuda' or dtype != torch.bfloat16):
+            raise ValueError('8-bit projections need CUDA and a bfloat16 decoder')
         self.cfg = cfg
+        self.fp8 = projections == 'fp8'
         gen = torch.Generator(device='cpu').manual_seed(seed)
 
         def w(*shape):
             return torch.nn.Parameter((torch.randn(*shape, generator=gen) * cfg.init_std).to(dtype).to(device),
                                       requires_grad=False)
 
+        def per_layer(*shape):  # the same random weights whatever they are held in
+            weights = (w(*shape) for _ in range(cfg.layers))
+            if self.fp8:
+                return torch.nn.ModuleList([Fp8Weight(x) for x in weights])
+            return torch.nn.ParameterList(list(weights))
+
         qkv_out = (cfg.q_heads + 2 * cfg.kv_heads) * cfg.head_dim
         self.embed = w(cfg.vocab, cfg.hidden)
-        self.qkv = torch.nn.ParameterList([w(qkv_out, cfg.hidden) for _ in range(cfg.layers)])
-        self.o = torch.nn.ParameterList([w(cfg.hidden, cfg.q_heads * cfg.head_dim) for _ in range(cfg.layers)])
-        self.gate_up = torch.nn.ParameterList([w(2 * cfg.intermediate, cfg.hidden) for _ in range(cfg.layers)])
-        self.down = torch.nn.ParameterList([w(cfg.hidden, cfg.intermediate) for _ in range(cfg.layers)])
+        self.qkv = per_layer(qkv_out, cfg.hidden)
+        self.o = per_layer(cfg.hidden, cfg.q_heads * cfg.head_dim)
+        if self.fp8:  # gate and up apart: each one's blocks begin at its own first row
+            self.gate, self.up = torch.nn.ModuleList(), torch.nn.ModuleList()
+            for _ in range(cfg.layers):
+                gate, up = w(2 * cfg.intermediate, cfg.hidden).chunk(2)
+                self.gate.append(Fp8Weight(gate))
+                self.up.append(Fp8Weight(up))
+        else:
+            self.gate_up = per_layer(2 * cfg.intermediate, cfg.hidden)
+        self.down = per_layer(cfg.hidden, cfg.intermediate)
         ones = lambda: torch.nn.Parameter(torch.ones(cfg.hidden, dtype=dtype, device=device), requires_grad=False)
         self.norm_attn = torch.nn.ParameterList([ones() for _ in range(cfg.layers)])
         self.norm_mlp = torch.nn.ParameterList([ones() for _ in range(cfg.layers)])
@@ -100,8 +140,22 @@ class Decoder(torch.nn.Module):
 
     def add_norm(self, x, y, weight):
         """(x + y, its RMSNorm * weight): the residual add and the next norm of a
-        layer in one call (one launch on CUDA); y None: (x, norm of x)."""
-        return add_rms(x, y, weight, self.cfg.rms_eps)
+        layer in one call (one launch on CUDA); y None: (x, norm of x). With 8-bit
+        projections the norm is Fp8 rows."""
+        return (add_rms_fp8 if self.fp8 else add_rms)(x, y, weight, self.cfg.rms_eps)
+
+    def mlp(self, h, layer):
+        """The gated MLP of one layer's normed input h."""
+        if self.fp8:
+            return fp8_linear(fp8_gate_up(h, self.gate[layer].blocks, self.up[layer].blocks), self.down[layer].blocks)
+        gate, up = F.linear(h, self.gate_up[layer]).chunk(2, dim=-1)
+        return F.linear(activation_product(gate, up), self.down[layer])
+
+    def output(self, out, layer):
+        """The output projection of one layer's attention out [..., q_heads * head_dim]."""
+        if self.fp8:
+            return fp8_linear(fp8_quantize(out), self.o[layer].blocks)
+        return F.linear(out, self.o[layer])
 
     def run_layers(self, x, attend):
         """The decoder layers over x: attend(h, layer) is a layer's attention of the
@@ -110,8 +164,7 @@ class Decoder(torch.nn.Module):
         x, h = self.add_norm(x, None, self.norm_attn[0])
         for layer in range(c.layers):
             x, h = self.add_norm(x, attend(h, layer), self.norm_mlp[layer])
-            gate, up = F.linear(h, self.gate_up[layer]).chunk(2, dim=-1)
-            m = F.linear(activation_product(gate, up), self.down[layer])
+            m = self.mlp(h, layer)
             if layer + 1 < c.layers:
                 x, h = self.add_norm(x, m, self.norm_attn[layer + 1])
             else:
@@ -119,13 +172,14 @@ class Decoder(torch.nn.Module):
         return x
 
     def project_qkv(self, x, layer, cos, sin):
-        """q [B, q_heads, n, d] and k / v [B, kv_heads, n, d] of x [B, n, hidden]: one
-        joined projection and one rotary pass over the query and key heads together
+        """q [B, q_heads, n, d] and k / v [B, kv_heads, n, d] of x [B, n, hidden] (bf16,
+        or Fp8 rows with 8-bit projections): one joined projection and one rotary pass over the query and key heads together
         (cos / sin [B or 1, n, 1, d]); q, k and v are strided views, which the cache
         kernels take as they are."""
         c = self.cfg
-        b, n = x.shape[0], x.shape[1]
-        h = F.linear(x, self.qkv[layer]).view(b, n, c.q_heads + 2 * c.kv_heads, c.head_dim)
+        h = fp8_linear(x, self.qkv[layer].blocks) if self.fp8 else F.linear(x, self.qkv[layer])
+        b, n = h.shape[0], h.shape[1]
+        h = h.view(b, n, c.q_heads + 2 * c.kv_heads, c.head_dim)
         if h.is_cuda:  # one launch, bit-identical to apply_rope
             qk = K.rotary(h, cos, sin, c.q_heads + c.kv_heads)
         else:  # the native-cache decoder on the CPU
@@ -141,23 +195,23 @@ class Decoder(torch.nn.Module):
         return cos.view(b, n, 1, -1), sin.view(b, n, 1, -1)
 
     def attention(self, x, layer, cache, cos, sin):
-        n = x.shape[1]
         q, k, v = self.project_qkv(x, layer, cos, sin)
+        n = q.shape[2]
         if isinstance(cache, GPUCache):
             out = cache.append_attend(q, k, v, layer)  # append + attend in one call; [1, n, q_heads, d]
         else:
             past = cache.get_seq_length(layer)
             kk, vv = cache.update(k, v, layer)
-            mask = torch.arange(past + n, device=x.device)[None, :] <= past + torch.arange(n, device=x.device)[:, None]
+            mask = torch.arange(past + n, device=q.device)[None, :] <= past + torch.arange(n, device=q.device)[:, None]
             out = F.scaled_dot_product_attention(q, kk, vv, attn_mask=mask, enable_gqa=True).transpose(1, 2)
-        return F.linear(out.reshape(1, n, -1), self.o[layer])
+        return self.output(out.reshape(1, n, -1), layer)
 
     def attention_chunks(self, x, layer, cache, cos, sin):
         """Attention of B token chunks x [B, n, hidden] side by side over the cache's
         history: each chunk sees the history and its own earlier tokens; nothing is
         appended (the packed path runs one batched kernel call per layer)."""
-        b, n = x.shape[0], x.shape[1]
         q, k, v = self.project_qkv(x, layer, cos, sin)
+        b, n = q.shape[0], q.shape[2]
         past = cache.get_seq_length(layer)
         if isinstance(cache, GPUCache):
             out = cache.attend_batched(q, k, v, layer, past)  # [B, n, q_heads, d]
@@ -165,19 +219,19 @@ class Decoder(torch.nn.Module):
             if past:
                 k = torch.cat((cache.k[layer].expand(b, -1, -1, -1), k), 2)
                 v = torch.cat((cache.v[layer].expand(b, -1, -1, -1), v), 2)
-            mask = torch.arange(past + n, device=x.device)[None, :] <= past + torch.arange(n, device=x.device)[:, None]
+            mask = torch.arange(past + n, device=q.device)[None, :] <= past + torch.arange(n, device=q.device)[:, None]
             out = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, enable_gqa=True).transpose(1, 2)
-        return F.linear(out.reshape(b, n, -1), self.o[layer])
+        return self.output(out.reshape(b, n, -1), layer)
 
     def attention_many(self, x, layer, caches, cos, sin):
         """Attention of B requests' frames x [B, n, hidden], request r over caches[r],
         appending each frame's K/V to its own cache (one pack and one attention
         launch for all of them)."""
-        b, n = x.shape[0], x.shape[1]
         q, k, v = self.project_qkv(x, layer, cos, sin)
+        b, n = q.shape[0], q.shape[2]
         pasts = append_many(caches, k, v, layer)
         out = attend_many(caches, q, k, v, layer, pasts)  # [B, n, q_heads, d]
-        return F.linear(out.reshape(b, n, -1), self.o[layer])
+        return self.output(out.reshape(b, n, -1), layer)
 
     def forward_many(self, caches, ids=None, embeds=None, logits=0):
         """forward() for B independent requests stepped together (request batching,
@@ -208,7 +262,7 @@ class Decoder(torch.nn.Module):
 
         def attend(h, layer):
             q, k, v = self.project_qkv(h, layer, cos, sin)
-            out = torch.empty((b, n, c.q_heads, c.head_dim), dtype=h.dtype, device=h.device)
+            out = torch.empty((b, n, c.q_heads, c.head_dim), dtype=q.dtype, device=q.device)
             if batch.append:
                 K.append_attention_many_device(q, k, v, batch.targets_ptr, batch.histories_ptr, b, batch.max_past,
                                                out, layer, n, c.kv_heads, c.q_heads // c.kv_heads, c.head_dim,
@@ -216,7 +270,7 @@ class Decoder(torch.nn.Module):
             else:
                 K.packed_attention_many_device(q, k, v, batch.histories_ptr, b, batch.max_past, out, layer, n,
                                                c.kv_heads, c.q_heads // c.kv_heads, c.head_dim, c.layers)
-            return F.linear(out.reshape(b, n, -1), self.o[layer])
+            return self.output(out.reshape(b, n, -1), layer)
 
         x = self.run_layers(x, attend)
         if not logits:

@@ -5,7 +5,8 @@ Keeps the reference CLI's switches (src/inference.py:9-14): --mode
 --device. The reference reads a video and a checkpoint; this build has neither,
 so a request is a seeded stand-in (random-init SmolLM2-360M-shape decoder, frame
 embeddings, question and four candidates, see streaming.synthetic_request). All
-modes need the GPU runtime; there is no CPU path.
+modes need the GPU runtime; there is no CPU path. --projections fp8 (not in the
+reference) holds the decoder's projection weights and their inputs in 8 bits.
 
     python -m src.inference --mode dynamic --frames 16
 """
@@ -15,7 +16,7 @@ import time
 
 import torch
 
-from .decoder import SMOLLM2_360M
+from .decoder import PROJECTIONS, SMOLLM2_360M
 from .gpu_cache import GPUCache
 from .streaming import MODES, StreamingModel, bits_for, synthetic_request
 
@@ -26,6 +27,7 @@ def parse(argv=None):
     p.add_argument('--mode', choices=MODES, default='dynamic')
     p.add_argument('--device', choices=['auto', 'cpu', 'cuda'], default='auto')
     p.add_argument('--frames', type=int)
+    p.add_argument('--projections', choices=PROJECTIONS, default='bf16')
     args = p.parse_args(argv)
     if args.frames is not None and not 1 <= args.frames <= 96:
         p.error('--frames must be between 1 and 96')
@@ -59,7 +61,7 @@ def main(argv=None):
     args = parse(argv)
     if args.device == 'cpu' or not torch.cuda.is_available():
         raise RuntimeError('This mode requires the GPU runtime')
-    model = StreamingModel(SMOLLM2_360M, device='cuda')
+    model = StreamingModel(SMOLLM2_360M, device='cuda', projections=args.projections)
     print(json.dumps(timed_request(model, args.sample, args.frames or 16, args.mode), indent=2))
 
 

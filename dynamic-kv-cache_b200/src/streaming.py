@@ -40,10 +40,10 @@ def bits_for(mode, frames, seed=0):
 
 
 class StreamingModel:
-    def __init__(self, cfg=SMOLLM2_360M, device='cuda', seed=0, prefix_tokens=11):
+    def __init__(self, cfg=SMOLLM2_360M, device='cuda', seed=0, prefix_tokens=11, projections='bf16'):
         self.cfg = cfg
         self.device = torch.device(device)
-        self.model = Decoder(cfg, device=device, seed=seed)
+        self.model = Decoder(cfg, device=device, seed=seed, projections=projections)
         gen = torch.Generator().manual_seed(seed + 1)
         self.prefix_ids = torch.randint(0, cfg.vocab, (1, prefix_tokens), generator=gen).to(self.device)
         self._frame_graphs = {}  # (requests, tokens, logits, append) -> FrameGraph, captured once and rebound
