@@ -29,12 +29,9 @@ namespace dkv {
 using namespace ptx;
 
 constexpr long long kGemmWaitCycles = 400000000LL;  // ~0.2 s: a healthy wait is microseconds
-constexpr int kGemmStages = 4;     // operand stages at most
-constexpr int kGemmSlots = 4;      // accumulators in TMEM, one column group each
 constexpr int kGemmThreads = 256;  // warps 0-3: scale and add; 4: copies; 5: MMA issue; all: the final sums
 constexpr int kTileRows = 128;     // weight rows of a tile
 constexpr int kMaxSplits = 16;
-constexpr int kMaxSmem = 228 * 1024 - 3 * 1536;  // of an SM, without the blocks' static and reserved parts
 
 struct GemmArgs {
   const float* sa;         // [m, groups]
@@ -53,10 +50,12 @@ struct GemmTile {
   static constexpr int kTokenBytes = NT * kFp8Group;
   static constexpr int kStageBytes = kParts * kWeightBytes + kTokenBytes;
   static constexpr int kCols = NT * kParts;  // TMEM columns of one accumulator
-  static constexpr int kTmemCols = kCols * kGemmSlots;
+  // Column groups in flight at most: operands in shared memory and an accumulator in TMEM each.
+  static constexpr int kStages = 4;
+  static constexpr int kTmemCols = kCols * 4;
   // blocks per SM: while one starts, loads or sums up, others keep the copies going
   static constexpr int kBlocks = kCols <= 32 ? 3 : 2;
-  static_assert(kParts * NT * kTileRows * 4 <= 2 * kStageBytes, "one block's sums fit the smallest operand ring");
+  static_assert(kParts * NT * kTileRows * 4 <= 3 * kStageBytes, "one block's sums fit the smallest operand ring");
   static_assert(kTmemCols * kBlocks <= 512 && kTmemCols >= 32 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM allocation");
   // operand ring, partial sums of `splits` blocks (one block's reuse the ring), scale products
   static int mail_bytes(int splits) {
@@ -83,7 +82,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
                 const __grid_constant__ CUtensorMap amap, const GemmArgs a) {
   using T = GemmTile<NT, GATE>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * kGemmStages + 2 * kGemmSlots + 1];
+  __shared__ __align__(8) uint64_t bars[3 * T::kStages + 1];
   __shared__ uint32_t tmem_slot;
   const uint32_t ring = (smem_addr(smem_raw) + 1023u) & ~1023u;
   uint8_t* const ring_ptr = smem_raw + (ring - smem_addr(smem_raw));
@@ -94,11 +93,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   const uint32_t mail = ring + a.stages * T::kStageBytes;
   float* const scales = reinterpret_cast<float*>(
       ring_ptr + a.stages * T::kStageBytes + (a.splits > 1 ? a.splits * T::kParts * local * kTileRows * 4 : 0));
-  const uint32_t full = smem_addr(bars);
-  const uint32_t empty = full + 8 * kGemmStages;
-  const uint32_t done = empty + 8 * kGemmStages;  // an accumulator is complete
-  const uint32_t freed = done + 8 * kGemmSlots;   // ... and read
-  const uint32_t mailed = freed + 8 * kGemmSlots; // the mail is complete
+  const uint32_t full = smem_addr(bars);        // a stage's operands are there
+  const uint32_t done = full + 8 * T::kStages;  // ... its products are done: accumulator complete, operands read
+  const uint32_t freed = done + 8 * T::kStages; // ... and the accumulator is read
+  const uint32_t mailed = freed + 8 * T::kStages;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -112,8 +110,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   const int mine = max(0, min(local, live - rank * local));  // tokens that this block adds up
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2 * kGemmStages + kGemmSlots; ++i) mbar_init(full + 8 * i, 1);
-    for (int i = 0; i < kGemmSlots; ++i) mbar_init(freed + 8 * i, 128);
+    for (int i = 0; i < 2 * T::kStages; ++i) mbar_init(full + 8 * i, 1);
+    for (int i = 0; i < T::kStages; ++i) mbar_init(freed + 8 * i, 4);  // one arrival per warp
     mbar_init(mailed, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -132,21 +130,29 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   if (a.splits > 1) cluster_arrive_release();  // this block has started: others may write to it
   pdl_wait();  // operands are the previous kernels' output
 
+  // Copies and products are issued by one thread each, whose every instruction waits for the
+  // last: the loops are unrolled over the stages, so that nothing but the waits, the issues
+  // and a few additions is left in them (with addresses and descriptors made on the way, the
+  // issuing took longer than the products).
   if (warp == 4) {
-    if (lane == 0) {
+    if (elect_one()) {
+      bool ok = true;
       int i = 0;
-      for (int s = 0, phase = 1; i < count; ++i) {
-        if (i >= a.stages && !mbar_wait(empty + 8 * s, phase, kGemmWaitCycles)) break;
-        const uint32_t dst = ring + s * T::kStageBytes;
-        const int x = (group0 + i) * kFp8Group;
-        mbar_arrive_expect_tx(full + 8 * s, T::kStageBytes);
-        tile2d_g2s(dst, &wmap, x, tile * kTileRows, full + 8 * s);
-        if (GATE) tile2d_g2s(dst + T::kWeightBytes, &umap, x, tile * kTileRows, full + 8 * s);
-        tile2d_g2s(dst + T::kParts * T::kWeightBytes, &amap, x, token0, full + 8 * s);
-        if (++s == a.stages) s = 0, phase ^= 1;
+      for (uint32_t phase = 1; i < count && ok; phase ^= 1) {
+#pragma unroll
+        for (int s = 0; s < T::kStages; ++s, ++i) {
+          if (i >= count || s == a.stages) break;
+          if (i >= a.stages) ok = mbar_wait(done + 8 * s, phase, kGemmWaitCycles);
+          if (!ok) break;
+          const uint32_t dst = ring + s * T::kStageBytes;
+          const int x = (group0 + i) * kFp8Group;
+          mbar_arrive_expect_tx(full + 8 * s, T::kStageBytes);
+          tile2d_g2s(dst, &wmap, x, tile * kTileRows, full + 8 * s);
+          if (GATE) tile2d_g2s(dst + T::kWeightBytes, &umap, x, tile * kTileRows, full + 8 * s);
+          tile2d_g2s(dst + T::kParts * T::kWeightBytes, &amap, x, token0, full + 8 * s);
+        }
       }
-      // a wait that ran out: the copies in flight still target this block's memory
-      if (i < count)
+      if (!ok)  // a wait that ran out: the copies in flight still target this block's memory
         for (int j = max(0, i - a.stages); j < i; ++j)
           mbar_wait(full + 8 * (j % a.stages), (j / a.stages) & 1, kGemmWaitCycles);
     }
@@ -161,26 +167,29 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     named_bar_arrive(2, 160);  // the products need not wait for the scales
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc = idesc_e4m3(kTileRows, NT);
-      for (int i = 0, s = 0, phase = 0; i < count; ++i) {
-        const int slot = i % kGemmSlots;
-        bool ok = mbar_wait(full + 8 * s, phase, kGemmWaitCycles);
-        if (ok && i >= kGemmSlots) ok = mbar_wait(freed + 8 * slot, ((i / kGemmSlots) + 1) & 1, kGemmWaitCycles);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t src = ring + s * T::kStageBytes;
-        const uint64_t wd = sw128_desc(src, 16, 1024);
-        const uint64_t ud = sw128_desc(src + T::kWeightBytes, 16, 1024);
-        const uint64_t ad = sw128_desc(src + T::kParts * T::kWeightBytes, 16, 1024);
+      const uint64_t wd0 = sw128_desc(ring, 16, 1024);
+      const uint64_t ud0 = wd0 + (T::kWeightBytes >> 4);
+      const uint64_t ad0 = wd0 + (T::kParts * T::kWeightBytes >> 4);
+      bool ok = true;
+      int i = 0;
+      for (uint32_t phase = 0; i < count && ok; phase ^= 1) {
 #pragma unroll
-        for (int j = 0; j < kFp8Group / 32; ++j) {  // 32 columns are 32 bytes: 2 descriptor units
-          umma_f8(tmem + slot * T::kCols, wd + 2 * j, ad + 2 * j, idesc, j > 0);
-          if (GATE) umma_f8(tmem + slot * T::kCols + NT, ud + 2 * j, ad + 2 * j, idesc, j > 0);
+        for (int s = 0; s < T::kStages; ++s, ++i) {
+          if (i >= count || s == a.stages) break;
+          ok = mbar_wait(full + 8 * s, phase, kGemmWaitCycles);
+          if (ok && i >= a.stages) ok = mbar_wait(freed + 8 * s, phase ^ 1, kGemmWaitCycles);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int j = 0; j < kFp8Group / 32; ++j) {  // 32 columns are 32 bytes: 2 descriptor units
+            const uint32_t at = s * (T::kStageBytes >> 4) + 2 * j;
+            umma_f8(tmem + s * T::kCols, wd0 + at, ad0 + at, idesc, j > 0);
+            if (GATE) umma_f8(tmem + s * T::kCols + NT, ud0 + at, ad0 + at, idesc, j > 0);
+          }
+          umma_commit(done + 8 * s);
         }
-        umma_commit(done + 8 * slot);
-        umma_commit(empty + 8 * s);
-        if (++s == a.stages) s = 0, phase ^= 1;
       }
     }
     __syncwarp();
@@ -204,9 +213,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     for (int j = 0; j < T::kCols; ++j) acc[j] = 0.f;
     const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
     bool ok = true;
-    for (int i = 0; i < count && ok; ++i) {
-      const int slot = i % kGemmSlots;
-      ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * slot, (i / kGemmSlots) & 1, kGemmWaitCycles));
+    for (int i = 0, slot = 0, phase = 0; i < count && ok; ++i) {
+      ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * slot, phase, kGemmWaitCycles));
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
@@ -228,7 +236,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
         }
       }
       tc_fence_before();
-      mbar_arrive(freed + 8 * slot);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(freed + 8 * slot);
+      if (++slot == a.stages) slot = 0, phase ^= 1;
     }
     // a wait that ran out leaves NaN, not a stale tile
 #pragma unroll
@@ -347,7 +357,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
 // GATE makes the halves the gate and the up rows of the same 128 intermediate columns:
 // each thread then holds matching columns of G and U.
 constexpr int kWideThreads = 384;  // warps 0-7: scale and add; 8: copies; 9: MMA issue; 10, 11: none
-constexpr int kWideStages = 5;
+constexpr int kWideStages = 4;
 constexpr int kWideHalf = 128 * kFp8Group;  // bytes of one block's operand tile of one group
 constexpr int kWideStageBytes = 2 * kWideHalf;
 constexpr int kWideChunk = 16;  // groups whose scales are staged at a time
@@ -455,63 +465,78 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   tc_fence_before();
   cluster_arrive_release();  // the copies need not wait for TMEM: their warps join at the end
 
-  // 384 x 168 registers at launch = 128 x (56 + 224 + 224)
+  // 384 x 168 registers at launch = 128 x (72 + 216 + 216)
   if (warp >= 8) {
-    regs_give<56>();
+    regs_give<72>();
     if (warp == 9) {
       cluster_wait_acquire();
       tc_fence_after();
       pdl_trigger();  // after every block's allocation
     }
-    if (warp == 8 && lane == 0) {
+    const int total = (tiles - pair + pairs - 1) / pairs * a.groups;  // groups of all tiles
+    if (warp == 8 && elect_one()) {
       const uint32_t full0 = dsmem_addr(full, 0);
-      int i = 0;
+      const CUtensorMap* const rows = GATE && rank == 1 ? &umap : &wmap;
+      int tile = pair, x = 0;
+      int token0 = (tile % tiles_m) * 256 + rank * 128;
+      int row0 = (tile / tiles_m) * kColumns + (GATE ? 0 : rank * 128);
       bool ok = true;
-      for (int tile = pair; tile < tiles && ok; tile += pairs) {
-        const int token0 = (tile % tiles_m) * 256 + rank * 128;
-        const int row0 = (tile / tiles_m) * kColumns + (GATE ? 0 : rank * 128);
-        for (int g = 0; g < a.groups; ++g, ++i) {
-          const int s = i % kWideStages;
-          if (i >= kWideStages && !mbar_wait(done + 8 * s, ((i / kWideStages) + 1) & 1, kGemmWaitCycles)) {
-            ok = false;
-            break;
-          }
+      int i = 0;
+      for (uint32_t phase = 1; i < total && ok; phase ^= 1) {
+#pragma unroll
+        for (int s = 0; s < kWideStages; ++s, ++i) {
+          if (i >= total) break;
+          if (i >= kWideStages) ok = mbar_wait(done + 8 * s, phase, kGemmWaitCycles);
+          if (!ok) break;
           const uint32_t dst = ring + s * kWideStageBytes;
           if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, 2 * kWideStageBytes);
-          tile2d_g2s_pair(dst, &amap, g * kFp8Group, token0, full0 + 8 * s);
-          tile2d_g2s_pair(dst + kWideHalf, GATE && rank == 1 ? &umap : &wmap, g * kFp8Group, row0, full0 + 8 * s);
+          tile2d_g2s_pair(dst, &amap, x, token0, full0 + 8 * s);
+          tile2d_g2s_pair(dst + kWideHalf, rows, x, row0, full0 + 8 * s);
+          x += kFp8Group;
+          if (x >= a.groups * kFp8Group) {
+            x = 0;
+            tile += pairs;
+            token0 = (tile % tiles_m) * 256 + rank * 128;
+            row0 = (tile / tiles_m) * kColumns + (GATE ? 0 : rank * 128);
+          }
         }
       }
       if (!ok && rank == 0)  // a wait that ran out: the copies in flight still target shared memory
         for (int j = max(0, i - kWideStages); j < i; ++j)
           mbar_wait(full + 8 * (j % kWideStages), (j / kWideStages) & 1, kGemmWaitCycles);
-    } else if (warp == 9 && rank == 1 && lane == 0) {
-      const int total = (tiles - pair + pairs - 1) / pairs * a.groups;
+    } else if (warp == 9 && rank == 1 && elect_one()) {
+      // one arrival in the other block's shared memory costs as much as many in this one's
       const uint32_t freed0 = dsmem_addr(freed, 0);
       for (int i = 0; i < total; ++i) {
         const int slot = i % kWideSlots;
         if (!mbar_wait(freed + 8 * slot, (i / kWideSlots) & 1, kGemmWaitCycles)) break;
         mbar_arrive_cluster(freed0 + 8 * slot);
       }
-    } else if (warp == 9 && rank == 0 && lane == 0) {
+    } else if (warp == 9 && rank == 0 && elect_one()) {
       constexpr uint32_t idesc = idesc_e4m3(256, kWideCols);
       const uint32_t tmem = tmem_slot;
-      const int total = (tiles - pair + pairs - 1) / pairs * a.groups;
+      const uint64_t ad0 = sw128_desc(ring, 16, 1024);
+      const uint64_t wd0 = ad0 + (kWideHalf >> 4);
       bool ok = true;
-      for (int i = 0; i < total && ok; ++i) {
-        const int s = i % kWideStages;
-        ok = mbar_wait(full + 8 * s, (i / kWideStages) & 1, kGemmWaitCycles);
-        const uint32_t src = ring + s * kWideStageBytes;
-        const uint64_t ad = sw128_desc(src, 16, 1024);
-        const uint64_t wd = sw128_desc(src + kWideHalf, 16, 1024);
-        const int slot = i % kWideSlots;
-        if (ok && i >= kWideSlots) ok = mbar_wait(freed + 8 * slot, ((i / kWideSlots) + 1) & 1, kGemmWaitCycles);
-        if (!ok) break;
-        tc_fence_after();
+      int i = 0;
+      static_assert(kWideStages == 2 * kWideSlots, "a stage uses accumulator s % 2, in its turn s / 2");
+      for (uint32_t phase = 0; i < total && ok; phase ^= 1) {
 #pragma unroll
-        for (int j = 0; j < kFp8Group / 32; ++j)
-          umma_f8_pair(tmem + slot * kWideCols, ad + 2 * j, wd + 2 * j, idesc, j > 0);
-        umma_commit_pair(done + 8 * s);
+        for (int s = 0; s < kWideStages; ++s, ++i) {
+          if (i >= total) break;
+          const int slot = s % kWideSlots;
+          ok = mbar_wait(full + 8 * s, phase, kGemmWaitCycles);
+          // an accumulator goes round twice while the stages go round once
+          if (ok && i >= kWideSlots) ok = mbar_wait(freed + 8 * slot, s < kWideSlots ? 1 : 0, kGemmWaitCycles);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int j = 0; j < kFp8Group / 32; ++j) {
+            const uint32_t at = s * (kWideStageBytes >> 4) + 2 * j;
+            umma_f8_pair(tmem + slot * kWideCols, ad0 + at, wd0 + at, idesc, j > 0);
+          }
+          umma_commit_pair(done + 8 * s);
+        }
       }
     }
     if (warp >= 10) {
@@ -548,7 +573,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     __syncwarp();
     if (warp != 9) cluster_wait_acquire();
   } else {
-    regs_take<224>();
+    regs_take<216>();
     cluster_wait_acquire();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
@@ -714,8 +739,9 @@ cudaError_t launch_gemm(const GemmCall& c, int splits, cudaStream_t stream) {
   GemmArgs args = c.args;
   args.splits = splits;
   const int per = (args.groups + splits - 1) / splits;
-  args.stages = per < 2 ? 2 : per < kGemmStages ? per : kGemmStages;
-  while (args.stages > 2 && T::smem(args.stages, splits, per) > kMaxSmem / T::kBlocks) --args.stages;
+  // one more stage where blocks have an SM to themselves; two or three share it otherwise
+  const int64_t blocks = static_cast<int64_t>((args.n + kTileRows - 1) / kTileRows) * splits * ((args.m + NT - 1) / NT);
+  args.stages = blocks <= 148 ? T::kStages : 3;
   const int smem = T::smem(args.stages, splits, per);
   cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<NT, GATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e == cudaSuccess && splits > 8)
