@@ -19,8 +19,6 @@
 // so its scale is found in the tile.
 #include <cuda.h>
 
-#include <mutex>
-
 #include "fp8.cuh"
 #include "tc_ptx.cuh"
 
@@ -794,15 +792,16 @@ cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
 }
 
 // Which kernel, how many tokens per tile and how many blocks per tile: the least time by a
-// model fitted to a sweep of all of them over 34 shapes (1 to 8192 tokens, 128 to 49280
-// weight rows, 256 to 16384 columns; inputs beyond L2; us on a B200, the model within ~15 %):
-//   split kernel  2.4 + stream + sums, where one wave of blocks streams its operands at 62
-//                 bytes/ns per SM, and r waves take r * (0.9 + bytes / 85); the partial sums
-//                 of a split tile cross between SMs at 0.023 per token column
-//   pair kernel   4.2 + per wave of 74 tiles: 0.44 per column group + 1.7 (GATE: 2.2) per tile
-// Measured either side of its borders: 512 x 960 x 960 5.5 us by 32 tokens (64: 6.1, pairs
-// 9.5); 64 x 960 x 2560 4.4 by 32 tokens and 5 blocks a tile (one: 9.3); 2048 x 1600 x 960
-// 10.0 by pairs (64 tokens: 12.8).
+// model fitted to a sweep of all of them over 49 shapes (1 to 8192 tokens, 128 to 49280 weight
+// rows, 256 to 16384 columns; weights beyond L2; in us on a B200, mostly within 10 %). With c
+// the accumulator columns of a token tile (tokens, doubled by GATE):
+//   split kernel  start 2.0 + 0.012 c (GATE 0.5 more), 0.9 for every block an SM has to start
+//                 beyond its first; per column group 0.12 + 0.003 c, or the time in which all
+//                 blocks' operands come from L2 at 13 bytes/ps; summing up a split tile 0.3 + 0.02 c
+//   pair kernel   start 5.0; per wave of 74 tiles 0.42 per column group and 1.4 (GATE 2.1)
+// Measured on either side of its borders: 512 x 960 x 960 4.3 us by 32 tokens a tile (64: 5.3,
+// pairs 9.5); 64 x 960 x 2560 3.9 by 16 tokens and 3 blocks a tile (one: 5.6; 64 tokens and 5
+// blocks: 4.8); 2048 x 1600 x 960 10.5 by pairs (64 tokens: 11.7).
 struct GemmPlan {
   int tokens;  // per tile; 256: the pair kernel
   int splits;
@@ -813,11 +812,12 @@ GemmPlan make_gemm_plan(int m, int n, int groups, bool gate) {
   const int wide_columns = gate ? 128 : 256;
   const int64_t wide_tiles = static_cast<int64_t>((m + 255) / 256) * ((n + wide_columns - 1) / wide_columns);
   GemmPlan best{256, 1};
-  float least = 4.2f + static_cast<float>((wide_tiles + 73) / 74) * (groups * 0.44f + (gate ? 2.2f : 1.7f));
+  float least = 5.0f + static_cast<float>((wide_tiles + 73) / 74) * (groups * 0.42f + (gate ? 2.1f : 1.4f));
   for (int nt = 16; nt <= (gate ? 32 : 64); nt *= 2) {
     const int64_t tiles = static_cast<int64_t>((n + kTileRows - 1) / kTileRows) * ((m + nt - 1) / nt);
     if (tiles > INT32_MAX / kMaxSplits || (m + nt - 1) / nt > 65535) continue;
-    const float stage = (parts * kTileRows + nt) * kFp8Group * 1e-3f;
+    const float columns = static_cast<float>(nt * parts);
+    const float stage = (parts * kTileRows + nt) * kFp8Group * 1e-6f / 13.f;  // us per block at 13 bytes/ps
     for (int s = 1; s <= kMaxSplits && s <= groups; ++s) {
       const int per = (groups + s - 1) / s;
       if ((groups + per - 1) / per != s) continue;  // a block would have nothing to do
@@ -825,14 +825,11 @@ GemmPlan make_gemm_plan(int m, int n, int groups, bool gate) {
       // blocks that start at once, one per SM: clusters stay within a GPC, of which there are
       // eight of at least 16 SMs, and sizes that do not divide 16 pack less tightly
       const float room = s == 1 ? 148.f : 16 % s == 0 ? 128.f : 0.9f * 8 * (18 / s) * s;
-      float time = 2.4f + (s > 1 ? 0.023f * nt * parts : 0.f);
-      if (blocks <= room) {
-        time += per * stage / 62.f;
-      } else {
-        float waves = 2.f;  // two blocks share an SM
-        if (blocks > 2 * room) waves = s == 1 ? blocks / 148.f : 2.f * static_cast<int>((blocks + 2 * room - 1) / (2 * room));
-        time += waves * (0.9f + per * stage / 85.f);
-      }
+      float group = 0.12f + 0.003f * columns;
+      if (blocks * stage > group) group = blocks * stage;
+      float time = 2.0f + 0.012f * columns + (gate ? 0.5f : 0.f) + per * group;
+      if (s > 1) time += 0.3f + 0.02f * columns + (blocks > 2 * room ? 0.2f * per * group : 0.f);
+      if (blocks > room) time += 0.9f * (blocks > 296 ? blocks / 148.f - 1 : 1.f);
       if (time < least) {
         least = time;
         best = {nt, s};
