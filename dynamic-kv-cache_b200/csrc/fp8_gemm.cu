@@ -460,8 +460,13 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     tmem_alloc_pair(smem_addr(&tmem_slot), kWideTmem);
     tmem_relinquish_pair();
   }
+  // The copies need not wait for TMEM: their warps join at the end. Only the allocating warp
+  // has something to release (a release waits for the thread's memory operations).
   tc_fence_before();
-  cluster_arrive_release();  // the copies need not wait for TMEM: their warps join at the end
+  if (warp == 9)
+    cluster_arrive_release();
+  else
+    cluster_arrive_relaxed();
 
   // 384 x 168 registers at launch = 128 x (72 + 216 + 216)
   if (warp >= 8) {
@@ -557,14 +562,16 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
             ok = false;
             break;
           }
-          float* dst = scales + (c & 1) * kWideScales;
-          const float* src = a.sa + static_cast<int64_t>(token0) * a.groups + g0;
+          // asynchronous 4-byte copies: all of them in flight at once, and none in registers
+          const uint32_t dst = smem_addr(scales + (c & 1) * kWideScales);
           const int g = t % kWideChunk;
-          if (g < n)
-            for (int token = t / kWideChunk; token < tokens; token += 64 / kWideChunk)
-              dst[g * 128 + token] = __ldg(src + static_cast<int64_t>(token) * a.groups + g);
-          if (t < 2 * n) dst[kWideChunk * 128 + t] = __ldg((t & 1 ? sw1 : sw0) + g0 + (t >> 1));
-          mbar_arrive(staged + 8 * (c & 1));
+          if (g < n) {
+            const float* src = a.sa + (static_cast<int64_t>(token0) + t / kWideChunk) * a.groups + g0 + g;
+            for (int token = t / kWideChunk; token < tokens; token += 64 / kWideChunk, src += 64 / kWideChunk * a.groups)
+              cp_async4(dst + (g * 128 + token) * 4, src);
+          }
+          if (t < 2 * n) cp_async4(dst + (kWideChunk * 128 + t) * 4, (t & 1 ? sw1 : sw0) + g0 + (t >> 1));
+          cp_async_mbar_arrive(staged + 8 * (c & 1));
         }
       }
     }
@@ -679,8 +686,11 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       }
     }
   }
+  // the other block's copies, arrivals and products are done with this one (no memory to order:
+  // a release would wait for this block's stores)
   tc_fence_before();
-  cluster_sync_all();  // the other block's copies, arrivals and products are done with this one
+  cluster_arrive_relaxed();
+  cluster_wait_acquire();
   if (warp == 9) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_slot, kWideTmem);
