@@ -455,34 +455,35 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     prefetch_tensor_map(&amap);
   }
   cluster_sync_all();  // both blocks' barriers exist
-  pdl_wait();
-  if (warp == 9) {  // after the wait, before the trigger: see fp8_gemm_kernel
-    tmem_alloc_pair(smem_addr(&tmem_slot), kWideTmem);
-    tmem_relinquish_pair();
-  }
-  // The copies need not wait for TMEM: their warps join at the end. Only the allocating warp
-  // has something to release (a release waits for the thread's memory operations).
-  tc_fence_before();
-  if (warp == 9)
-    cluster_arrive_release();
-  else
-    cluster_arrive_relaxed();
+  const int total = (tiles - pair + pairs - 1) / pairs * a.groups;  // groups of all tiles
 
-  // 384 x 168 registers at launch = 128 x (72 + 216 + 216)
+  // 384 x 168 registers at launch = 128 x (72 + 216 + 216). Each role gets ready, and waits for
+  // the previous kernel, whose output the operands are, right before its first access.
   if (warp >= 8) {
     regs_give<72>();
     if (warp == 9) {
+      // TMEM is taken after the wait and before the trigger (see fp8_gemm_kernel). The blocks'
+      // rendezvous after it is relaxed: a release at cluster scope would take ~0.5 us, and
+      // what follows it are tcgen05 operations, fenced on both sides.
+      pdl_wait();
+      tmem_alloc_pair(smem_addr(&tmem_slot), kWideTmem);
+      tmem_relinquish_pair();
+      tc_fence_before();
+      named_bar_arrive(2, 288);  // the epilogue warps may read TMEM's address
+    }
+    cluster_arrive_relaxed();
+    if (warp == 9) {
       cluster_wait_acquire();
       tc_fence_after();
-      pdl_trigger();  // after every block's allocation
+      pdl_trigger();  // after both blocks' allocation
     }
-    const int total = (tiles - pair + pairs - 1) / pairs * a.groups;  // groups of all tiles
     if (warp == 8 && elect_one()) {
       const uint32_t full0 = dsmem_addr(full, 0);
       const CUtensorMap* const rows = GATE && rank == 1 ? &umap : &wmap;
       int tile = pair, x = 0;
       int token0 = (tile % tiles_m) * 256 + rank * 128;
       int row0 = (tile / tiles_m) * kColumns + (GATE ? 0 : rank * 128);
+      pdl_wait();
       bool ok = true;
       int i = 0;
       for (uint32_t phase = 1; i < total && ok; phase ^= 1) {
@@ -543,6 +544,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       }
     }
     if (warp >= 10) {
+      pdl_wait();
       // The scales arrive as rows of groups, and each epilogue thread needs one row: read by
       // that thread, every group would be 32 cache lines per warp. Copied flat and turned
       // over in shared memory, it is one conflict-free load.
@@ -579,7 +581,9 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     if (warp != 9) cluster_wait_acquire();
   } else {
     regs_take<216>();
-    cluster_wait_acquire();
+    cluster_arrive_relaxed();
+    pdl_wait();
+    named_bar_sync(2, 288);
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     const int part = warp >> 2;
@@ -688,6 +692,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   }
   // the other block's copies, arrivals and products are done with this one (no memory to order:
   // a release would wait for this block's stores)
+  if (warp < 8) cluster_wait_acquire();
   tc_fence_before();
   cluster_arrive_relaxed();
   cluster_wait_acquire();
