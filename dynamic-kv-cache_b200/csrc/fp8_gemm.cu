@@ -360,54 +360,59 @@ constexpr int kWideHalf = 128 * kFp8Group;  // bytes of one block's operand tile
 constexpr int kWideStageBytes = 2 * kWideHalf;
 constexpr int kWideChunk = 16;  // groups whose scales are staged at a time
 constexpr int kWideScales = kWideChunk * 128 + 2 * kWideChunk;  // [group][token], then [group][half] of the weights
-constexpr int kWideSmem = 1024 + kWideStages * kWideStageBytes + 2 * kWideScales * 4 + 8 * 32 * 128;
+constexpr int kTurnBytes = 32 * 128;  // of output: 32 tokens x 128 bytes
+constexpr int kWideSmem = 1024 + kWideStages * kWideStageBytes + 8 * 2 * kTurnBytes + 2 * kWideScales * 4;
 constexpr int kWideCols = 256;
 constexpr int kWideSlots = 2;
 constexpr uint32_t kWideTmem = kWideSlots * kWideCols;
 
-// A warp's tile leaves through its piece of shared memory: 32 tokens (one per lane) x 128 bytes,
-// written a row per lane and read back 8 lanes to a row, so that every store instruction fills
-// whole 128-byte lines (a row per lane would touch 32 of them, 16 or 32 bytes each). The
-// 16-byte pieces of row r are exchanged by r % 8: both directions are free of bank conflicts.
-constexpr int kTurnBytes = 32 * 128;
-
-__device__ __forceinline__ uint32_t turn_at(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
-
-// Writes `BYTES` (64 or 128) per token, as 16-byte words w, to row `token` (a row is `stride`
-// bytes) from byte `at` on, up to the row's end; rows from `tokens` on are left alone.
-// Rows that do not start on 16 bytes are stored element by element (SIZE bytes each).
-template <int BYTES, int SIZE>
-__device__ __forceinline__ void store_turned(uint8_t* out, int token, int tokens, int64_t stride, int64_t at,
-                                             const uint4* w, uint8_t* turn) {
+// A warp's output leaves through one of its two pieces of shared memory: 32 tokens (one per
+// lane) x BYTES (64 or 128), as 16-byte words w, in the swizzled order of a tensor map's box of
+// the same shape (word c of row r is exchanged by r % 8, with 64-byte rows by (r / 2) % 4: free
+// of bank conflicts), and from there as one tile copy that runs on while the warp goes on
+// (stores by the threads, in whole lines or not, held the epilogue up by 1000 clocks per 64
+// columns: every byte passes the shared memory and the store path of the SM).
+template <int BYTES>
+__device__ __forceinline__ void store_tile(const CUtensorMap* map, int x, int y, bool inside, const uint4* w,
+                                           uint8_t* piece) {
   const int lane = threadIdx.x & 31;
-  constexpr int kPieces = BYTES / 16;
+  if (lane == 0) bulk_wait_read<1>();  // the tile before last has left this piece
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < BYTES / 16; ++c) {
+    const int at = BYTES == 128 ? c ^ (lane & 7) : c ^ ((lane >> 1) & 3);
+    *reinterpret_cast<uint4*>(piece + lane * BYTES + at * 16) = w[c];
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    if (inside) tile2d_s2g(map, x, y, smem_addr(piece));
+    bulk_commit();
+  }
+}
+
+// The same for rows that no tensor map can describe (a row's start not on 16 bytes): the lanes
+// store neighbouring elements of a row, SIZE bytes each; rows from `tokens` on are left alone.
+template <int SIZE>
+__device__ __forceinline__ void store_elements(uint8_t* out, int token, int tokens, int64_t stride, int64_t at,
+                                               const uint4* w, uint8_t* piece) {
+  const int lane = threadIdx.x & 31;
   __syncwarp();  // the last call's reads
 #pragma unroll
-  for (int c = 0; c < kPieces; ++c) *reinterpret_cast<uint4*>(turn + turn_at(lane, c)) = w[c];
+  for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(piece + lane * 128 + ((c ^ (lane & 7)) << 4)) = w[c];
   __syncwarp();
-  const int first = token - lane;
-  if (stride % 16 == 0) {
-    const int c = lane % kPieces;
-#pragma unroll
-    for (int r = lane / kPieces; r < 32; r += 32 / kPieces) {
-      if (first + r < tokens && at + c * 16 < stride)
-        *reinterpret_cast<uint4*>(out + (first + r) * stride + at + c * 16) =
-            *reinterpret_cast<const uint4*>(turn + turn_at(r, c));
-    }
-  } else {
 #pragma unroll 4
-    for (int r = 0; r < 32; ++r) {
-      if (first + r >= tokens) break;
+  for (int r = 0; r < 32; ++r) {
+    if (token - lane + r >= tokens) break;
 #pragma unroll
-      for (int b = lane * SIZE; b < BYTES; b += 32 * SIZE) {
-        const uint8_t* src = turn + turn_at(r, b >> 4) + (b & 15);
-        uint8_t* dst = out + (first + r) * stride + at + b;
-        if (at + b >= stride) break;
-        if constexpr (SIZE == 4) {
-          *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
-        } else {
-          *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
-        }
+    for (int b = lane * SIZE; b < 128; b += 32 * SIZE) {
+      const uint8_t* src = piece + r * 128 + (((b >> 4) ^ (r & 7)) << 4) + (b & 15);
+      uint8_t* dst = out + (token - lane + r) * stride + at + b;
+      if (at + b >= stride) break;
+      if constexpr (SIZE == 4) {
+        *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+      } else {
+        *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
       }
     }
   }
@@ -416,7 +421,7 @@ __device__ __forceinline__ void store_turned(uint8_t* out, int token, int tokens
 template <bool GATE>
 __global__ void __launch_bounds__(kWideThreads, 1)
 fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap umap,
-                const __grid_constant__ CUtensorMap amap, const GemmArgs a) {
+                const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap omap, const GemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[2 * kWideStages + kWideSlots + 4];
   __shared__ uint32_t tmem_slot;
@@ -429,7 +434,8 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   const uint32_t freed = done + 8 * kWideStages;  // rank 0's: both blocks have read an accumulator
   const uint32_t staged = freed + 8 * kWideSlots;  // each block's own: a chunk of scales is there
   const uint32_t used = staged + 16;               // ... and no longer needed
-  float* const scales = reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)) + kWideStages * kWideStageBytes);
+  uint8_t* const pieces = smem_raw + (ring - smem_addr(smem_raw)) + kWideStages * kWideStageBytes;  // 1024-byte aligned
+  float* const scales = reinterpret_cast<float*>(pieces + 8 * 2 * kTurnBytes);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -589,7 +595,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     const int part = warp >> 2;
     const int token_in = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    uint8_t* const turn = reinterpret_cast<uint8_t*>(scales + 2 * kWideScales) + warp * kTurnBytes;
+    uint8_t* const turn = pieces + warp * 2 * kTurnBytes;
     int i = 0, chunk = 0;
     bool ok = true;
     const auto next_chunk = [&] {  // this warp is done with a chunk of scales
@@ -667,16 +673,23 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
         uint4 w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = codes16(acc + 16 * j, inverse);
-        store_turned<64, 1>(static_cast<uint8_t*>(a.out), token, a.m, a.n, col0, w, turn);  // n is a multiple of 16
+        // n is a multiple of 16: a tensor map describes every output
+        store_tile<64>(&omap, col0, token - lane, col0 < a.n && token - lane < a.m, w, turn + parity * kTurnBytes);
         if (live && part == 0) a.out_scale[static_cast<int64_t>(token) * blocks + tn] = __fdiv_rn(amax, kFp8Max);
       } else if (a.out_f32) {
 #pragma unroll
-        for (int j = 0; j < 128; j += 32)
-          store_turned<128, 4>(static_cast<uint8_t*>(a.out), token, a.m, 4LL * a.n, 4LL * (tn * 256 + part * 128 + j),
-                               reinterpret_cast<const uint4*>(acc + j), turn);
+        for (int j = 0; j < 128; j += 32) {
+          const int col = tn * 256 + part * 128 + j;
+          const uint4* w = reinterpret_cast<const uint4*>(acc + j);
+          if (a.n % 4 == 0)
+            store_tile<128>(&omap, col, token - lane, col < a.n && token - lane < a.m, w, turn + (j / 32 & 1) * kTurnBytes);
+          else
+            store_elements<4>(static_cast<uint8_t*>(a.out), token, a.m, 4LL * a.n, 4LL * col, w, turn);
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 128; j += 64) {
+          const int col = tn * 256 + part * 128 + j;
           uint4 w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -684,11 +697,14 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
             w[i] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
                               pack_bf16x2(v[6], v[7]));
           }
-          store_turned<128, 2>(static_cast<uint8_t*>(a.out), token, a.m, 2LL * a.n, 2LL * (tn * 256 + part * 128 + j), w,
-                               turn);
+          if (a.n % 8 == 0)
+            store_tile<128>(&omap, col, token - lane, col < a.n && token - lane < a.m, w, turn + (j / 64) * kTurnBytes);
+          else
+            store_elements<2>(static_cast<uint8_t*>(a.out), token, a.m, 2LL * a.n, 2LL * col, w, turn);
         }
       }
     }
+    if (lane == 0) bulk_wait_read<0>();  // the pieces are read; the grid ends when all is written
   }
   // the other block's copies, arrivals and products are done with this one (no memory to order:
   // a release would wait for this block's stores)
@@ -731,6 +747,26 @@ bool encode_tiles(CUtensorMap* map, const void* base, int64_t rows, int64_t cols
   const cuuint32_t steps[2] = {1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, boxes, steps,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The output's tiles of 32 rows x 128 bytes (e4m3: 64) as store_tile writes them; an output whose
+// rows do not start on 16 bytes has none, and its map is not used.
+bool encode_output(CUtensorMap* map, const GemmArgs& a, bool gate) {
+  const FnEncode fn = encoder();
+  if (fn == nullptr) return false;
+  const int size = gate ? 1 : a.out_f32 ? 4 : 2;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.n), static_cast<cuuint64_t>(a.m)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a.n) * size};
+  if (strides[0] % 16 != 0) return true;
+  const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(gate ? 64 : 128 / size), 32};
+  const cuuint32_t steps[2] = {1, 1};
+  return fn(map,
+            gate        ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+            : a.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+            2, a.out, dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            gate ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -779,10 +815,11 @@ cudaError_t launch_gemm(const GemmCall& c, int splits, cudaStream_t stream) {
 
 template <bool GATE>
 cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
-  CUtensorMap wmap, umap, amap;
+  CUtensorMap wmap, umap, amap, omap = {};
   if (!encode_tiles(&wmap, c.w, c.args.n, c.k, c.ws, 128) || !encode_tiles(&amap, c.a, c.args.m, c.k, c.as, 128))
     return cudaErrorInvalidValue;
   umap = wmap;
+  if (!encode_output(&omap, c.args, GATE)) return cudaErrorInvalidValue;
   if (GATE && !encode_tiles(&umap, c.u, c.args.n, c.k, c.us, 128)) return cudaErrorInvalidValue;
   const cudaError_t e =
       cudaFuncSetAttribute(fp8_wide_kernel<GATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
@@ -803,7 +840,7 @@ cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, fp8_wide_kernel<GATE>, wmap, umap, amap, c.args);
+  return cudaLaunchKernelEx(&cfg, fp8_wide_kernel<GATE>, wmap, umap, amap, omap, c.args);
 }
 
 // Which kernel, how many tokens per tile and how many blocks per tile: the least time by a

@@ -122,6 +122,25 @@ __device__ __forceinline__ void tile2d_prefetch(const void* map, int x, int y) {
                : "memory");
 }
 
+// Shared memory to a tile of a tensor (what lies outside is not written); completion by groups
+// of the issuing thread. Generic writes of the source are fenced first (fence_proxy_async_smem).
+__device__ __forceinline__ void tile2d_s2g(const void* map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(map), "r"(x),
+               "r"(y), "r"(src)
+               : "memory");
+}
+
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
+
+// Waits until all but this thread's N latest groups have been read from shared memory.
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory");
+}
+
+// ... until all groups are written.
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
+
 // tile2d_g2s from a block of a CTA pair: `bar` may lie in the other block (dsmem_addr).
 __device__ __forceinline__ void tile2d_g2s_pair(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
   asm volatile(
