@@ -275,18 +275,25 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     if (mine > 0) complete = mbar_wait(mailed, 0, kGemmWaitCycles);
   }
 
-  // a warp per token, 4 weight rows (output columns) per lane
-  const int col = tile * kTileRows + lane * 4;
+  // A warp per token, 4 weight rows (output columns) per lane: neighbouring ones where a row's
+  // start lets them be stored together, else every 32nd, so that neighbouring lanes store
+  // neighbouring columns.
+  const bool vectors = GATE || (a.n & 3) == 0;
+  const int col = tile * kTileRows + (vectors ? lane * 4 : lane);
   const int first = a.splits > 1 ? rank * local : 0;
+  const auto take = [&](const float* at) {
+    at += vectors ? lane * 4 : lane;
+    return vectors ? *reinterpret_cast<const float4*>(at) : make_float4(at[0], at[32], at[64], at[96]);
+  };
   for (int i = warp; i < (a.splits > 1 ? mine : live); i += kGemmThreads / 32) {
     const int t = first + i;
     float4 sum[T::kParts];
 #pragma unroll
     for (int p = 0; p < T::kParts; ++p) {
-      const float* at = sums + p * parts_apart + i * kTileRows + lane * 4;
-      sum[p] = *reinterpret_cast<const float4*>(at);
+      const float* at = sums + p * parts_apart + i * kTileRows;
+      sum[p] = take(at);
       for (int r = 1; r < a.splits; ++r) {
-        const float4 v = *reinterpret_cast<const float4*>(at + r * T::kParts * parts_apart);
+        const float4 v = take(at + r * T::kParts * parts_apart);
         sum[p].x += v.x;
         sum[p].y += v.y;
         sum[p].z += v.z;
@@ -312,26 +319,24 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     } else {
       const float4 v = sum[0];
       const int64_t at = row * a.n + col;
-      const bool whole = col + 4 <= a.n && (a.n & 3) == 0;
+      const float e[4] = {v.x, v.y, v.z, v.w};
       if (a.out_f32) {
         float* o = static_cast<float*>(a.out) + at;
-        if (whole) {
-          *reinterpret_cast<float4*>(o) = v;
+        if (vectors) {
+          if (col < a.n) *reinterpret_cast<float4*>(o) = v;
         } else {
-          if (col < a.n) o[0] = v.x;
-          if (col + 1 < a.n) o[1] = v.y;
-          if (col + 2 < a.n) o[2] = v.z;
-          if (col + 3 < a.n) o[3] = v.w;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (col + 32 * j < a.n) o[32 * j] = e[j];
         }
       } else {
         __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + at;
-        if (whole) {
-          *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+        if (vectors) {
+          if (col < a.n) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
         } else {
-          if (col < a.n) o[0] = __float2bfloat16_rn(v.x);
-          if (col + 1 < a.n) o[1] = __float2bfloat16_rn(v.y);
-          if (col + 2 < a.n) o[2] = __float2bfloat16_rn(v.z);
-          if (col + 3 < a.n) o[3] = __float2bfloat16_rn(v.w);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (col + 32 * j < a.n) o[32 * j] = __float2bfloat16_rn(e[j]);
         }
       }
     }
@@ -391,34 +396,52 @@ __device__ __forceinline__ void store_tile(const CUtensorMap* map, int x, int y,
   }
 }
 
-// The same for rows that no tensor map can describe (a row's start not on 16 bytes): the lanes
-// store neighbouring elements of a row, SIZE bytes each; rows from `tokens` on are left alone.
+// The same for rows that no tensor map can describe (a row's start not on 16 bytes): a lane
+// stores one aligned 4-byte word of a row, the warp a row at a time, eight rows read at once. A
+// bf16 row that starts between words is shifted by one element, its ends stored alone. Rows
+// from `tokens` on and columns from `columns` on (of the warp's `128 / SIZE`) are left alone;
+// `out` is the first row's first column, rows are n elements apart.
 template <int SIZE>
-__device__ __forceinline__ void store_elements(uint8_t* out, int token, int tokens, int64_t stride, int64_t at,
-                                               const uint4* w, uint8_t* piece) {
+__device__ __forceinline__ void store_words(uint8_t* out, int64_t n, bool odd_start, int tokens, int columns,
+                                            const uint4* w, uint8_t* piece) {
   const int lane = threadIdx.x & 31;
   __syncwarp();  // the last call's reads
 #pragma unroll
   for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(piece + lane * 128 + ((c ^ (lane & 7)) << 4)) = w[c];
   __syncwarp();
-#pragma unroll 4
-  for (int r = 0; r < 32; ++r) {
-    if (token - lane + r >= tokens) break;
+  if (columns <= 0) return;
+#pragma unroll 1
+  for (int r0 = 0; r0 < 32 && r0 < tokens; r0 += 8) {
+    uint32_t v[8];
 #pragma unroll
-    for (int b = lane * SIZE; b < 128; b += 32 * SIZE) {
-      const uint8_t* src = piece + r * 128 + (((b >> 4) ^ (r & 7)) << 4) + (b & 15);
-      uint8_t* dst = out + (token - lane + r) * stride + at + b;
-      if (at + b >= stride) break;
+    for (int i = 0; i < 8; ++i)
+      v[i] = *reinterpret_cast<const uint32_t*>(piece + (r0 + i) * 128 + (((lane >> 2) ^ i) << 4) + (lane & 3) * 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool row = r0 + i < tokens;
+      uint8_t* dst = out + (r0 + i) * n * SIZE;
       if constexpr (SIZE == 4) {
-        *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+        if (row && lane < columns) reinterpret_cast<uint32_t*>(dst)[lane] = v[i];
       } else {
-        *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
+        const uint32_t next = __shfl_down_sync(0xffffffffu, v[i], 1);
+        const int c = 2 * lane;
+        uint16_t* e = reinterpret_cast<uint16_t*>(dst);
+        if (!odd_start == !((r0 + i) & n & 1)) {  // the row starts on a word
+          if (row && c + 1 < columns) *reinterpret_cast<uint32_t*>(e + c) = v[i];
+          if (row && c + 1 == columns) e[c] = static_cast<uint16_t>(v[i]);
+        } else {
+          if (row && c + 2 < columns && lane < 31) *reinterpret_cast<uint32_t*>(e + c + 1) = (v[i] >> 16) | (next << 16);
+          if (row && c + 1 < columns && (c + 2 == columns || lane == 31)) e[c + 1] = static_cast<uint16_t>(v[i] >> 16);
+          if (row && lane == 0) e[0] = static_cast<uint16_t>(v[i]);
+        }
       }
     }
   }
 }
 
-template <bool GATE>
+// WORDS: the output's rows do not start on 16 bytes (a kernel of its own: its stores cost the
+// other one registers in the loop over the groups).
+template <bool GATE, bool WORDS>
 __global__ void __launch_bounds__(kWideThreads, 1)
 fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap umap,
                 const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap omap, const GemmArgs a) {
@@ -681,10 +704,11 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
         for (int j = 0; j < 128; j += 32) {
           const int col = tn * 256 + part * 128 + j;
           const uint4* w = reinterpret_cast<const uint4*>(acc + j);
-          if (a.n % 4 == 0)
+          if constexpr (!WORDS)
             store_tile<128>(&omap, col, token - lane, col < a.n && token - lane < a.m, w, turn + (j / 32 & 1) * kTurnBytes);
           else
-            store_elements<4>(static_cast<uint8_t*>(a.out), token, a.m, 4LL * a.n, 4LL * col, w, turn);
+            store_words<4>(static_cast<uint8_t*>(a.out) + (static_cast<int64_t>(token - lane) * a.n + col) * 4, a.n, false,
+                           a.m - (token - lane), a.n - col, w, turn);
         }
       } else {
 #pragma unroll
@@ -697,10 +721,11 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
             w[i] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
                               pack_bf16x2(v[6], v[7]));
           }
-          if (a.n % 8 == 0)
+          if constexpr (!WORDS)
             store_tile<128>(&omap, col, token - lane, col < a.n && token - lane < a.m, w, turn + (j / 64) * kTurnBytes);
           else
-            store_elements<2>(static_cast<uint8_t*>(a.out), token, a.m, 2LL * a.n, 2LL * col, w, turn);
+            store_words<2>(static_cast<uint8_t*>(a.out) + (static_cast<int64_t>(token - lane) * a.n + col) * 2, a.n,
+                           (static_cast<int64_t>(token - lane) * a.n + col) & 1, a.m - (token - lane), a.n - col, w, turn);
         }
       }
     }
@@ -813,7 +838,7 @@ cudaError_t launch_gemm(const GemmCall& c, int splits, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<NT, GATE>, wmap, umap, amap, args);
 }
 
-template <bool GATE>
+template <bool GATE, bool WORDS>
 cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
   CUtensorMap wmap, umap, amap, omap = {};
   if (!encode_tiles(&wmap, c.w, c.args.n, c.k, c.ws, 128) || !encode_tiles(&amap, c.a, c.args.m, c.k, c.as, 128))
@@ -822,7 +847,7 @@ cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
   if (!encode_output(&omap, c.args, GATE)) return cudaErrorInvalidValue;
   if (GATE && !encode_tiles(&umap, c.u, c.args.n, c.k, c.us, 128)) return cudaErrorInvalidValue;
   const cudaError_t e =
-      cudaFuncSetAttribute(fp8_wide_kernel<GATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+      cudaFuncSetAttribute(fp8_wide_kernel<GATE, WORDS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
   if (e != cudaSuccess) return e;
   const int columns = GATE ? 128 : 256;
   const int64_t tiles = static_cast<int64_t>((c.args.m + 255) / 256) * ((c.args.n + columns - 1) / columns);
@@ -840,7 +865,7 @@ cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, fp8_wide_kernel<GATE>, wmap, umap, amap, omap, c.args);
+  return cudaLaunchKernelEx(&cfg, fp8_wide_kernel<GATE, WORDS>, wmap, umap, amap, omap, c.args);
 }
 
 // Which kernel, how many tokens per tile and how many blocks per tile: the least time by a
@@ -850,10 +875,10 @@ cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
 //   split kernel  start 2.0 + 0.012 c (GATE 0.5 more), 0.9 for every block an SM has to start
 //                 beyond its first; per column group 0.12 + 0.003 c, or the time in which all
 //                 blocks' operands come from L2 at 13 bytes/ps; summing up a split tile 0.3 + 0.02 c
-//   pair kernel   start 5.0; per wave of 74 tiles 0.42 per column group and 1.4 (GATE 2.1)
+//   pair kernel   start 3.0; per wave of 74 tiles 0.40 per column group and 1.2 (GATE 2.0)
 // Measured on either side of its borders: 512 x 960 x 960 4.3 us by 32 tokens a tile (64: 5.3,
-// pairs 9.5); 64 x 960 x 2560 3.9 by 16 tokens and 3 blocks a tile (one: 5.6; 64 tokens and 5
-// blocks: 4.8); 2048 x 1600 x 960 10.5 by pairs (64 tokens: 11.7).
+// pairs 7.3); 64 x 960 x 2560 3.9 by 16 tokens and 3 blocks a tile (one: 5.6; 64 tokens and 5
+// blocks: 4.8); 2048 x 1600 x 960 8.1 by pairs (64 tokens: 11.7).
 struct GemmPlan {
   int tokens;  // per tile; 256: the pair kernel
   int splits;
@@ -864,7 +889,7 @@ GemmPlan make_gemm_plan(int m, int n, int groups, bool gate) {
   const int wide_columns = gate ? 128 : 256;
   const int64_t wide_tiles = static_cast<int64_t>((m + 255) / 256) * ((n + wide_columns - 1) / wide_columns);
   GemmPlan best{256, 1};
-  float least = 5.0f + static_cast<float>((wide_tiles + 73) / 74) * (groups * 0.42f + (gate ? 2.1f : 1.4f));
+  float least = 3.0f + static_cast<float>((wide_tiles + 73) / 74) * (groups * 0.40f + (gate ? 2.0f : 1.2f));
   for (int nt = 16; nt <= (gate ? 32 : 64); nt *= 2) {
     const int64_t tiles = static_cast<int64_t>((n + kTileRows - 1) / kTileRows) * ((m + nt - 1) / nt);
     if (tiles > INT32_MAX / kMaxSplits || (m + nt - 1) / nt > 65535) continue;
@@ -899,7 +924,10 @@ cudaError_t launch_planned(const GemmCall& c, cudaStream_t stream) {
     case 16: return launch_gemm<16, GATE>(c, p.splits, stream);
     case 32: return launch_gemm<32, GATE>(c, p.splits, stream);
     case 64: return launch_gemm<GATE ? 32 : 64, GATE>(c, p.splits, stream);
-    default: return launch_wide<GATE>(c, stream);
+    default:
+      if (GATE || static_cast<int64_t>(c.args.n) * (c.args.out_f32 ? 4 : 2) % 16 == 0)
+        return launch_wide<GATE, false>(c, stream);
+      return launch_wide<GATE, !GATE>(c, stream);
   }
 }
 
