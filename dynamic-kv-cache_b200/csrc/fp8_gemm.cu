@@ -64,14 +64,29 @@ struct GemmTile {
   }
 };
 
-// silu(g) * u = g / (1 + 2^(-g log2 e)) * u on the special-function unit: 2^x and 1 / x are off
-// by a few fp32 units, and the exponent's rounding by |g| of them, far under the 2^-4 of the
-// rounding to e4m3 that follows (IEEE expf and division made the epilogue the bottleneck).
-// Where 2^x overflows, 1 / inf = 0 and the result is the 0 that silu tends to.
-__device__ __forceinline__ float silu_times(float g, float u) {
+// h = silu(g) * u of four values, with e = 2^(-|g| log2 e) <= 1 and d = 1 + e in [1, 2]:
+// silu(g) = g / d for g >= 0 and g e / d below, which neither overflows nor loses small results.
+// The four quotients share one reciprocal of d0 d1 d2 d3: the special-function unit, a quarter
+// of a result per clock and lane group, is what bounds this epilogue (five uses here; a power
+// and a reciprocal each took 2048 clocks per 128 x 128 tile, IEEE expf and division more). Off
+// by a few fp32 units (the exponent's rounding by |g| of them), far under the 2^-4 of the
+// rounding to e4m3 that follows. A NaN spreads within its column group, whose scale is NaN.
+__device__ __forceinline__ void silu_times4(const float* g, const float* u, float* h) {
+  float num[4], d[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float e = ex2(-1.4426950408889634f * fabsf(g[j]));
+    d[j] = 1.0f + e;
+    num[j] = (g[j] < 0.f ? g[j] * e : g[j]) * u[j];
+  }
+  const float d01 = d[0] * d[1], d23 = d[2] * d[3];
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(1.0f + ex2(-1.4426950408889634f * g)));
-  return g * r * u;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(d01 * d23));
+  const float r01 = r * d23, r23 = r * d01;  // 1 / d01, 1 / d23
+  h[0] = num[0] * (r01 * d[1]);
+  h[1] = num[1] * (r01 * d[0]);
+  h[2] = num[2] * (r23 * d[3]);
+  h[3] = num[3] * (r23 * d[2]);
 }
 
 template <int NT, bool GATE>
@@ -303,10 +318,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     }
     const int64_t row = token0 + t;
     if (GATE) {  // n is a multiple of 16: a lane's 4 columns are all inside or all outside
-      const float4 g = sum[0], u = sum[T::kParts - 1];
       float4 h = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (col < a.n)
-        h = make_float4(silu_times(g.x, u.x), silu_times(g.y, u.y), silu_times(g.z, u.z), silu_times(g.w, u.w));
+      if (col < a.n) silu_times4(&sum[0].x, &sum[T::kParts - 1].x, &h.x);
       float amax = max_nan(max_nan(fabsf(h.x), fabsf(h.y)), max_nan(fabsf(h.z), fabsf(h.w)));
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
@@ -683,9 +696,9 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
         for (int j = 0; j < 64; j += 16) {
           float m = 0.f;
 #pragma unroll
-          for (int i = j; i < j + 16; ++i) {
-            acc[i] = silu_times(acc[i], acc[64 + i]);
-            m = max_nan(m, fabsf(acc[i]));
+          for (int i = j; i < j + 16; i += 4) {
+            silu_times4(acc + i, acc + 64 + i, acc + i);
+            m = max_nan(m, max_nan(max_nan(fabsf(acc[i]), fabsf(acc[i + 1])), max_nan(fabsf(acc[i + 2]), fabsf(acc[i + 3]))));
           }
           if (j < inside) amax = max_nan(amax, m);
         }
