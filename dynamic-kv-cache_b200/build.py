@@ -54,7 +54,7 @@ def build_binding(verbose=False):
            *[f'-I{p}' for p in ce.include_paths(device_type='cuda')],
            str(BINDING_SOURCE), '-o', str(tmp), '-L', str(HERE), '-ldkv', "-Wl,-rpath,$ORIGIN",
            *[f'-L{p}' for p in ce.library_paths(device_type='cuda')],
-           '-lc10', '-lc10_cuda', '-ltorch', '-ltorch_cpu', '-ltorch_python', '-lcudart']
+           '-lc10', '-lc10_cuda', '-ltorch', '-ltorch_cpu', '-ltorch_cuda', '-ltorch_python', '-lcudart']
     if verbose:
         print(' '.join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)

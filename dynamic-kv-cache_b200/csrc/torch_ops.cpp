@@ -6,6 +6,7 @@
 // kernels from Python once per layer (src/gpu_cache.py:90-92, 99-103), so this host
 // cost is paid on every layer of every frame.
 #include <torch/extension.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -248,6 +249,12 @@ int64_t rows_of(const at::Tensor& x) { return x.size(-1) ? x.numel() / x.size(-1
 
 int32_t narrow(int64_t v) { return v > INT32_MAX ? INT32_MAX : static_cast<int32_t>(v); }
 
+// An uninitialised tensor on x's device, as at::empty makes it, without the dispatcher's
+// round (two or three of them were a quarter of a call's host time).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& x) {
+  return at::detail::empty_cuda(sizes, type, x.device(), c10::nullopt);
+}
+
 float* fp(const at::Tensor& t) { return static_cast<float*>(t.data_ptr()); }
 
 }  // namespace
@@ -258,8 +265,8 @@ std::vector<at::Tensor> fp8_quantize(const at::Tensor& x_in) {
   const at::Tensor x = bf16_rows(x_in, "fp8_quantize", &xs);
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t width = x.size(-1);
-  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-  at::Tensor s = at::empty(with_last(x, groups_of(width)), x.options().dtype(at::kFloat));
+  at::Tensor q = fresh(x.sizes(), at::kFloat8_e4m3fn, x);
+  at::Tensor s = fresh(with_last(x, groups_of(width)), at::kFloat, x);
   check(dkv_fp8_quantize(x.data_ptr(), q.data_ptr(), fp(s), rows_of(x), narrow(width), xs, current_stream(x)));
   return {q, s};
 }
@@ -271,8 +278,8 @@ std::vector<at::Tensor> fp8_quantize_weight(const at::Tensor& w_in) {
   const at::Tensor w = bf16_rows(w_in, "fp8_quantize_weight", &ws);
   const c10::cuda::CUDAGuard guard(w.device());
   const int64_t n = w.size(0), k = w.size(1);
-  at::Tensor q = at::empty({n, k}, w.options().dtype(at::kFloat8_e4m3fn));
-  at::Tensor s = at::empty({groups_of(n), groups_of(k)}, w.options().dtype(at::kFloat));
+  at::Tensor q = fresh({n, k}, at::kFloat8_e4m3fn, w);
+  at::Tensor s = fresh({groups_of(n), groups_of(k)}, at::kFloat, w);
   check(dkv_fp8_quantize_weight(w.data_ptr(), q.data_ptr(), fp(s), narrow(n), narrow(k), ws, current_stream(w)));
   return {q, s};
 }
@@ -292,10 +299,10 @@ std::vector<at::Tensor> add_rms_norm_fp8(const at::Tensor& x_in, const c10::opti
     if (y_in->sizes() != x.sizes() || y_in->device() != x.device())
       throw pybind11::value_error("add_rms_norm_fp8: y must match x");
     y = bf16_rows(*y_in, "add_rms_norm_fp8", &ys);
-    x_out = at::empty(x.sizes(), x.options());
+    x_out = fresh(x.sizes(), at::kBFloat16, x);
   }
-  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-  at::Tensor s = at::empty(with_last(x, groups_of(width)), x.options().dtype(at::kFloat));
+  at::Tensor q = fresh(x.sizes(), at::kFloat8_e4m3fn, x);
+  at::Tensor s = fresh(with_last(x, groups_of(width)), at::kFloat, x);
   check(dkv_add_rms_norm_fp8(x.data_ptr(), y.defined() ? y.data_ptr() : nullptr,
                              y.defined() ? x_out.data_ptr() : nullptr, q.data_ptr(), fp(s), w.data_ptr(), rows_of(x),
                              narrow(width), xs, ys, width, static_cast<float>(eps), current_stream(x)));
@@ -312,7 +319,7 @@ at::Tensor fp8_linear(const at::Tensor& q_in, const at::Tensor& s_in, const at::
     throw pybind11::value_error("fp8_linear: rows and weights must share their device and width");
   const c10::cuda::CUDAGuard guard(q.device());
   const int64_t n = w.size(0), k = w.size(1);
-  at::Tensor out = at::empty(with_last(q, n), q.options().dtype(out_f32 ? at::kFloat : at::kBFloat16));
+  at::Tensor out = fresh(with_last(q, n), out_f32 ? at::kFloat : at::kBFloat16, q);
   check(dkv_fp8_linear(q.data_ptr(), fp(s), w.data_ptr(), fp(wsc), out.data_ptr(), out_f32 ? 32 : 16, rows_of(q),
                        narrow(n), narrow(k), as, wstride, current_stream(q)));
   return out;
@@ -330,8 +337,8 @@ std::vector<at::Tensor> fp8_gate_up(const at::Tensor& q_in, const at::Tensor& s_
     throw pybind11::value_error("fp8_gate_up: gate and up must have one shape [n, width] on the rows' device");
   const c10::cuda::CUDAGuard guard(q.device());
   const int64_t n = g.size(0), k = g.size(1);
-  at::Tensor out = at::empty(with_last(q, n), q.options());
-  at::Tensor scale = at::empty(with_last(q, groups_of(n)), s.options());
+  at::Tensor out = fresh(with_last(q, n), at::kFloat8_e4m3fn, q);
+  at::Tensor scale = fresh(with_last(q, groups_of(n)), at::kFloat, q);
   check(dkv_fp8_gate_up(q.data_ptr(), fp(s), g.data_ptr(), fp(gsc), u.data_ptr(), fp(usc), out.data_ptr(), fp(scale),
                         rows_of(q), narrow(n), narrow(k), as, gstride, ustride, current_stream(q)));
   return {out, scale};
