@@ -30,6 +30,8 @@ constexpr long long kGemmWaitCycles = 400000000LL;  // ~0.2 s: a healthy wait is
 constexpr int kGemmThreads = 256;  // warps 0-3: scale and add; 4: copies; 5: MMA issue; all: the final sums
 constexpr int kTileRows = 128;     // weight rows of a tile
 constexpr int kMaxSplits = 16;
+constexpr int kMaxGroups = 16384 / kFp8Group;  // of the widest rows
+constexpr int kMaxGemmSmem = 210 * 1024;  // dynamic shared memory of any plan
 
 struct GemmArgs {
   const float* sa;         // [m, groups]
@@ -54,6 +56,10 @@ struct GemmTile {
   // blocks per SM: while one starts, loads or sums up, others keep the copies going
   static constexpr int kBlocks = kCols <= 32 ? 3 : 2;
   static_assert(kParts * NT * kTileRows * 4 <= 3 * kStageBytes, "one block's sums fit the smallest operand ring");
+  static_assert(1024 + kStages * kStageBytes + kParts * NT * 4 * kMaxGroups <= kMaxGemmSmem, "whole tiles");
+  static_assert(1024 + kStages * kStageBytes +
+                        kParts * 4 * ((NT + kMaxSplits - 1) * kTileRows + NT * ((kMaxGroups + 1) / 2)) <= kMaxGemmSmem,
+                "split tiles: sums of every rank's share, rounded up, and half of the scales at most");
   static_assert(kTmemCols * kBlocks <= 512 && kTmemCols >= 32 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM allocation");
   // operand ring, partial sums of `splits` blocks (one block's reuse the ring), scale products
   static int mail_bytes(int splits) {
@@ -830,7 +836,9 @@ cudaError_t launch_gemm(const GemmCall& c, int splits, cudaStream_t stream) {
   const int64_t blocks = static_cast<int64_t>((args.n + kTileRows - 1) / kTileRows) * splits * ((args.m + NT - 1) / NT);
   args.stages = blocks <= 148 ? T::kStages : 3;
   const int smem = T::smem(args.stages, splits, per);
-  cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<NT, GATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // the same limit for every call: threads that launch other shapes at the same time set it too
+  cudaError_t e =
+      cudaFuncSetAttribute(fp8_gemm_kernel<NT, GATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxGemmSmem);
   if (e == cudaSuccess && splits > 8)
     e = cudaFuncSetAttribute(fp8_gemm_kernel<NT, GATE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;

@@ -331,3 +331,81 @@ def test_refusals(cuda):
         with pytest.raises(ValueError, match=text):
             call()
     torch.cuda.synchronize()
+
+
+# Products with tokens enough for the pair kernel (256 x 256 tiles; more than 74 of them are several
+# rounds of the grid): rows and columns that end inside a tile, column groups of every remainder, and
+# every start of a row that the stores tell apart (n modulo 2, 4 and 8; bf16 and fp32).
+PAIRS = [(4096, 4096, 256), (3000, 4104, 144), (2049, 5000, 272), (2305, 4098, 400), (2500, 4097, 1040),
+         (5000, 2051, 528), (8192, 2052, 32), (2048, 2600, 2064)]
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('m,n,k', PAIRS)
+def test_linear_by_pairs(cuda, m, n, k, dtype):
+    gen = torch.Generator().manual_seed(m + n + k)
+    a, w = _rows(gen, m, k), _blocks(gen, n, k)
+    out = G.fp8_linear(a, w, dtype)
+    F.check_product(out, a, w)
+    assert torch.equal(G.fp8_linear(a, w, dtype), out)
+
+
+@pytest.mark.parametrize('m,n,k', [(4096, 2560, 960), (3001, 2576, 272), (2304, 1040, 2064), (700, 6416, 400)])
+def test_gate_up_by_pairs(cuda, m, n, k):
+    gen = torch.Generator().manual_seed(m + n + k)
+    a, gate, up = _rows(gen, m, k), _blocks(gen, n, k), _blocks(gen, n, k)
+    out = G.fp8_gate_up(a, gate, up)
+    F.check_gate_up(out, a, gate, up)
+    assert _same(G.fp8_gate_up(a, gate, up), out)
+
+
+@pytest.mark.parametrize('n,dtype', [(4096, torch.bfloat16), (4097, torch.bfloat16), (4102, torch.bfloat16),
+                                     (4096, torch.float32), (4099, torch.float32)])
+def test_pairs_keep_rows_and_columns_apart(cuda, n, dtype):
+    """NaN rows and a NaN weight block beside clean ones, in the middle of a larger buffer."""
+    from src import gpu_kernels as K
+    gen = torch.Generator().manual_seed(n)
+    m, k = 2500, 272
+    (q, s), (wq, ws) = _rows(gen, m, k), _blocks(gen, n, k)
+    ref = G.fp8_linear((q, s), (wq, ws), dtype)
+    s[::3], ws[3, 1] = float('nan'), float('nan')
+    pad = 1 << 15  # keeps the output's start on 16 bytes
+    flat = torch.full((m * n + 2 * pad,), 7.0, device='cuda', dtype=dtype)
+    out = flat[pad:pad + m * n].view(m, n)
+    rc = K.LIB.dkv_fp8_linear(q.data_ptr(), s.data_ptr(), wq.data_ptr(), ws.data_ptr(), out.data_ptr(),
+                              out.element_size() * 8, m, n, k, k, k, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, K.LIB.dkv_last_error()
+    torch.cuda.synchronize()
+    assert (flat[:pad] == 7).all() and (flat[pad + m * n:] == 7).all()
+    assert torch.isnan(out[::3]).all() and torch.isnan(out[:, 384:512]).all()
+    clean = torch.ones(m, dtype=torch.bool, device='cuda')
+    clean[::3] = False
+    keep = torch.ones(n, dtype=torch.bool, device='cuda')
+    keep[384:512] = False
+    assert torch.equal(out[clean][:, keep], ref[clean][:, keep])
+
+
+def test_threads_launch_different_shapes_at_once(cuda):
+    """Four host threads, each on its own stream with its own shapes: no call changes another's."""
+    import threading
+    shapes = [(1, 1600, 960), (64, 960, 2560), (512, 960, 960), (2048, 1600, 960)]
+    gen = torch.Generator().manual_seed(11)
+    operands = [(_rows(gen, m, k), _blocks(gen, n, k)) for m, n, k in shapes]
+    expected = [G.fp8_linear(*o) for o in operands]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                out = G.fp8_linear(*operands[i])
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(out, expected[i]):
+                    failed.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(shapes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
