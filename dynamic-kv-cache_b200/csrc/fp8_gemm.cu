@@ -8,11 +8,21 @@
 // two scales and added to the running sum in registers, in fp32, while the tensor cores
 // work on the next groups.
 //
-// fp8_gemm_kernel puts the weights on the 128 lanes of the accumulator and NT tokens on its
-// columns: the weights are what a decoder step has to stream, a tile holds 128 of their rows
-// whatever the token count, and 16 to 64 tokens waste no tensor work on padding. The column
-// groups of one tile are divided among the S blocks of a cluster when the tiles alone would
-// leave SMs idle; their partial sums meet in distributed shared memory, added in rank order.
+// fp8_gemm_kernel (few tokens) puts the weights on the 128 lanes of the accumulator and NT
+// tokens on its columns: the weights are what a decoder step has to stream, a tile holds 128 of
+// their rows whatever the token count, and 16 to 64 tokens waste little tensor work on padding.
+// The column groups of one tile are divided among the S blocks of a cluster when the tiles
+// alone would leave SMs idle; their partial sums cross by bulk copies between the SMs' shared
+// memories and are added in rank order. Small calls are bound by latency, a chain of the
+// previous kernel's end (~1 us), the first copies (~0.5), the products (~0.2), the scaling
+// (0.1 to 0.2 a group) and the sums and stores (0.3 to 0.8): 1 x 1600 x 960 2.75 us, 64 x 960 x
+// 2560 3.6, 333 x 1001 x 1040 5.4; many weight rows by memory: 25 x 49280 x 960 11.4 us, 4.6 of
+// 6.6 TB/s.
+//
+// fp8_wide_kernel (many tokens) is described below: 4096^3 64 us, 2.15 PFLOP/s, 65 % of twice
+// the measured bf16 rate (a plain library product of these e4m3 matrices, without block scales:
+// 49.5 us), bound by the round trip of an accumulator between the tensor cores and the threads
+// that scale it, and by 3.46 tiles per pair of SMs taking the time of 4.
 //
 // GATE computes two products with the same rows, G and U, and writes silu(g) * u as e4m3
 // rows: a tile of 128 intermediate columns is exactly one column group of the next product,
@@ -370,15 +380,18 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
 // fp8_wide_kernel keeps the tensor cores busy when there are tokens for it: a pair of
 // blocks works on a tile of 256 tokens x 256 weight rows, each block with 128 of the
 // tokens on its accumulators' lanes and half of the weight rows in its shared memory (so
-// per group and block 32 KB arrive for 2 x 128 x 256 x 128 products). A group's products go
-// to two accumulators of 128 columns, one per weight block of 128 rows; TMEM holds four, so
-// the tensor cores run up to two groups ahead of the eight epilogue warps that scale and
-// add them. A thread owns one token and 64 columns of each half: a half costs it one scale
-// product and 32 packed FMAs. The grid is persistent (one pair per two SMs): a tile's store
-// overlaps the next tile's first groups.
-// GATE makes the halves the gate and the up rows of the same 128 intermediate columns:
-// each thread then holds matching columns of G and U.
-constexpr int kWideThreads = 384;  // warps 0-7: scale and add; 8: copies; 9: MMA issue; 10, 11: none
+// per group and block 32 KB arrive for 128 x 256 x 128 products; blocks of their own would
+// need 48, and L2 gives an SM ~65 bytes per clock). Two accumulators of 256 columns fill
+// TMEM: while the tensor cores sum one group into one (512 clocks at their rate), the eight
+// epilogue warps scale and add the other. An accumulator's round (products, completion,
+// reading, release) takes ~1400 clocks, so two of them make a group ~700. Four accumulators of
+// 128 columns lost (products of 128 columns run at half rate: 96 us for 4096^3 against 67), as
+// did sixteen epilogue warps of 64 columns (72.6 against 70.3).
+// A thread owns one token and 128 columns; a group costs it a scale product and 64 packed FMAs.
+// The grid is persistent (one pair per two SMs): a tile's way out overlaps the next tile's first
+// groups. GATE gives the pair's first block the gate rows and the second the up rows of the
+// same 128 intermediate columns: each thread then holds matching columns of G and U.
+constexpr int kWideThreads = 384;  // warps 0-7: scale and add; 8: copies; 9: MMA issue; 10, 11: scales
 constexpr int kWideStages = 4;
 constexpr int kWideHalf = 128 * kFp8Group;  // bytes of one block's operand tile of one group
 constexpr int kWideStageBytes = 2 * kWideHalf;
@@ -471,7 +484,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   const uint32_t ring = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const uint32_t full = smem_addr(bars);         // rank 0's: both blocks' copies of a stage
   // each block's own: a stage's products are done, its accumulator complete and its buffers
-  // empty (one commit for both: a commit costs the issuing thread ~0.15 us)
+  // empty (one commit for both)
   const uint32_t done = full + 8 * kWideStages;
   const uint32_t freed = done + 8 * kWideStages;  // rank 0's: both blocks have read an accumulator
   const uint32_t staged = freed + 8 * kWideSlots;  // each block's own: a chunk of scales is there
@@ -490,7 +503,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * kWideStages; ++i) mbar_init(full + 8 * i, 1);
-    for (int i = 0; i < kWideSlots; ++i) mbar_init(freed + 8 * i, 8 + (rank == 0));  // the epilogue warps of both blocks
+    for (int i = 0; i < kWideSlots; ++i) mbar_init(freed + 8 * i, 8 + (rank == 0));  // own epilogue warps, and rank 1 as one
     for (int i = 0; i < 2; ++i) {
       mbar_init(staged + 8 * i, 64);
       mbar_init(used + 8 * i, 8);
@@ -557,7 +570,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
         for (int j = max(0, i - kWideStages); j < i; ++j)
           mbar_wait(full + 8 * (j % kWideStages), (j / kWideStages) & 1, kGemmWaitCycles);
     } else if (warp == 9 && rank == 1 && elect_one()) {
-      // one arrival in the other block's shared memory costs as much as many in this one's
+      // rank 1's eight warps reach rank 0 as one arrival
       const uint32_t freed0 = dsmem_addr(freed, 0);
       for (int i = 0; i < total; ++i) {
         const int slot = i % kWideSlots;

@@ -11,7 +11,9 @@
 // All are bound by memory: 2 bytes read and 1 + 4/128 written per element (the norm with a
 // residual reads 2 and writes 2 more). Every thread owns 16 consecutive columns: two 16-byte
 // loads, one 16-byte store, and a group of 128 columns is 8 neighbouring lanes, so its
-// maximum takes three shuffles.
+// maximum takes three shuffles. Measured: rows 8191 x 2560 10.1 us (6.3 of 6.6 TB/s), norm
+// 2048 x 8192 with a residual 18.9 us (6.2 TB/s), 8192 x 960 10.1 (5.5), without one 4097 x 4096
+// 10.0 (5.1); a decode step's single row is all latency, 1.5 and 2.0 us.
 #include "fp8.cuh"
 
 namespace dkv {
@@ -101,7 +103,7 @@ quantize_weight_kernel(const uint16_t* __restrict__ w, uint8_t* __restrict__ q, 
 // One row per WARPS warps at a time, two chunks of 16 columns per thread: width <= 1024 *
 // WARPS. Rows of one warp share a block of four. A block works through rows a grid apart: its
 // weights stay in registers, and the next row is on its way while this one is summed up, scaled
-// and stored (one row per block left the memory idle in between: 4097 x 4096 at 3.4 TB/s). A row
+// and stored (one row per block left the memory idle in between: 4097 x 4096 15.1 us). A row
 // is held as the bf16 it is (the residual sum is bf16 by definition), half the registers of
 // fp32. The sum of squares runs in fp32 in a fixed order (a thread's columns, a butterfly over
 // the warp, the warps in turn).

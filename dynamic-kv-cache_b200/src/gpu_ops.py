@@ -6,7 +6,8 @@ The GEMMs and the RMSNorm stay on PyTorch here; SiLU*up on CUDA bf16 tensors is
 one libdkv launch (dkv_silu_mul, bit-identical to the two PyTorch ops it
 replaces), and other dtypes / devices keep the reference's PyTorch form. The API
 and the weight-joining invariants (bit-identical parameter views over one joined
-tensor) are the same.
+tensor) are the same. Beside them stand the same steps in 8 bits (fp8_*,
+add_rms_fp8), where the projections are the library's own kernels too.
 """
 import types
 from typing import NamedTuple
