@@ -29,6 +29,8 @@
 // so its scale is found in the tile.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "fp8.cuh"
 #include "tc_ptx.cuh"
 
@@ -396,6 +398,7 @@ constexpr int kWideStages = 4;
 constexpr int kWideHalf = 128 * kFp8Group;  // bytes of one block's operand tile of one group
 constexpr int kWideStageBytes = 2 * kWideHalf;
 constexpr int kWideChunk = 16;  // groups whose scales are staged at a time
+constexpr int kWidePairs = 74;  // of blocks, all SMs
 constexpr int kWideScales = kWideChunk * 128 + 2 * kWideChunk;  // [group][token], then [group][half] of the weights
 constexpr int kTurnBytes = 32 * 128;  // of output: 32 tokens x 128 bytes
 constexpr int kWideSmem = 1024 + kWideStages * kWideStageBytes + 8 * 2 * kTurnBytes + 2 * kWideScales * 4;
@@ -471,9 +474,45 @@ __device__ __forceinline__ void store_words(uint8_t* out, int64_t n, bool odd_st
   }
 }
 
-// WORDS: the output's rows do not start on 16 bytes (a kernel of its own: its stores cost the
-// other one registers in the loop over the groups).
-template <bool GATE, bool WORDS>
+// How a pair kernel gives out its tiles and stores them: three kernels, because what the other
+// two need takes registers and clocks from the loop over the groups (one kernel for whole and half
+// tiles: 2048 x 4096 x 4096 34.8 us for 32.7; words in it: 4096 x 4097 x 4096 90 for 84).
+// kHalves: the last round's tiles, at most half as many as there are pairs, are cut into halves of
+// 128 weight rows. Products of 128 columns run at half rate (0.31 us a group for 0.40 of a whole
+// tile), but two pairs share a tile. GATE's tiles stay whole: a column group needs both halves.
+// kWords: the output's rows do not start on 16 bytes.
+enum class WideForm { kWhole, kHalves, kWords };
+
+WideForm wide_form(const GemmArgs& a, int64_t tiles, bool gate) {
+  if (gate) return WideForm::kWhole;
+  if (static_cast<int64_t>(a.n) * (a.out_f32 ? 4 : 2) % 16 != 0) return WideForm::kWords;
+  const int64_t rest = tiles % kWidePairs;
+  return rest > 0 && 2 * rest <= kWidePairs ? WideForm::kHalves : WideForm::kWhole;
+}
+
+// The tiles of one pair of blocks, `pairs` apart, first token fastest.
+template <bool HALVES>
+struct WideWork {
+  int pair, pairs, tiles_m, rounds, units;
+
+  __device__ __forceinline__ WideWork(const GemmArgs& a, int columns)
+      : pair(blockIdx.x >> 1), pairs(gridDim.x >> 1), tiles_m((a.m + 255) / 256) {
+    const int tiles = tiles_m * ((a.n + columns - 1) / columns);
+    rounds = tiles / pairs;
+    const int rest = tiles - rounds * pairs;
+    units = rounds + (pair < (HALVES ? 2 * rest : rest));
+  }
+  // Unit k: its first token, its tile of weight rows, and which half of it (-1: all).
+  __device__ __forceinline__ void unit(int k, int& token0, int& tn, int& half) const {
+    const bool cut = HALVES && k == rounds;
+    const int tile = k * pairs + (cut ? pair >> 1 : pair);
+    half = cut ? pair & 1 : -1;
+    token0 = (tile % tiles_m) * 256;
+    tn = tile / tiles_m;
+  }
+};
+
+template <bool GATE, WideForm FORM>
 __global__ void __launch_bounds__(kWideThreads, 1)
 fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap umap,
                 const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap omap, const GemmArgs a) {
@@ -495,11 +534,8 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int rank = blockIdx.x & 1;
-  const int pair = blockIdx.x >> 1;
-  const int pairs = gridDim.x >> 1;
-  constexpr int kColumns = GATE ? 128 : 256;  // output columns of a tile
-  const int tiles_m = (a.m + 255) / 256;
-  const int tiles = tiles_m * ((a.n + kColumns - 1) / kColumns);
+  constexpr bool kHalves = FORM == WideForm::kHalves;
+  const WideWork<kHalves> work(a, GATE ? 128 : 256);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * kWideStages; ++i) mbar_init(full + 8 * i, 1);
@@ -516,7 +552,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     prefetch_tensor_map(&amap);
   }
   cluster_sync_all();  // both blocks' barriers exist
-  const int total = (tiles - pair + pairs - 1) / pairs * a.groups;  // groups of all tiles
+  const int total = work.units * a.groups;  // groups of all tiles
 
   // 384 x 168 registers at launch = 128 x (72 + 216 + 216). Each role gets ready, and waits for
   // the previous kernel, whose output the operands are, right before its first access.
@@ -541,9 +577,14 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     if (warp == 8 && elect_one()) {
       const uint32_t full0 = dsmem_addr(full, 0);
       const CUtensorMap* const rows = GATE && rank == 1 ? &umap : &wmap;
-      int tile = pair, x = 0;
-      int token0 = (tile % tiles_m) * 256 + rank * 128;
-      int row0 = (tile / tiles_m) * kColumns + (GATE ? 0 : rank * 128);
+      int unit = 0, x = 0, token0, row0;
+      const auto next = [&] {  // a half tile's box holds 64 rows more than its products read
+        int tn, half;
+        work.unit(unit++, token0, tn, half);
+        token0 += rank * 128;
+        row0 = GATE ? tn * 128 : half < 0 ? tn * 256 + rank * 128 : tn * 256 + half * 128 + rank * 64;
+      };
+      next();
       pdl_wait();
       bool ok = true;
       int i = 0;
@@ -560,9 +601,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
           x += kFp8Group;
           if (x >= a.groups * kFp8Group) {
             x = 0;
-            tile += pairs;
-            token0 = (tile % tiles_m) * 256 + rank * 128;
-            row0 = (tile / tiles_m) * kColumns + (GATE ? 0 : rank * 128);
+            next();
           }
         }
       }
@@ -578,8 +617,8 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
         mbar_arrive_cluster(freed0 + 8 * slot);
       }
     } else if (warp == 9 && rank == 0 && elect_one()) {
-      constexpr uint32_t idesc = idesc_e4m3(256, kWideCols);
       const uint32_t tmem = tmem_slot;
+      const int cut = work.rounds * a.groups;  // from here on half tiles
       const uint64_t ad0 = sw128_desc(ring, 16, 1024);
       const uint64_t wd0 = ad0 + (kWideHalf >> 4);
       bool ok = true;
@@ -590,6 +629,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
         for (int s = 0; s < kWideStages; ++s, ++i) {
           if (i >= total) break;
           const int slot = s % kWideSlots;
+          const uint32_t idesc = !kHalves || i < cut ? idesc_e4m3(256, kWideCols) : idesc_e4m3(256, kWideCols / 2);
           ok = mbar_wait(full + 8 * s, phase, kGemmWaitCycles);
           // an accumulator goes round twice while the stages go round once
           if (ok && i >= kWideSlots) ok = mbar_wait(freed + 8 * slot, s < kWideSlots ? 1 : 0, kGemmWaitCycles);
@@ -612,9 +652,10 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       const int t = threadIdx.x - 32 * 10;
       int c = 0;
       bool ok = true;
-      for (int tile = pair; tile < tiles && ok; tile += pairs) {
-        const int token0 = (tile % tiles_m) * 256 + rank * 128;
-        const int tn = tile / tiles_m;
+      for (int unit = 0; unit < work.units && ok; ++unit) {
+        int token0, tn, half;
+        work.unit(unit, token0, tn, half);
+        token0 += rank * 128;
         const int tokens = min(128, a.m - token0);  // may be negative: nothing to read
         const float* sw0 = a.sw + static_cast<int64_t>(GATE ? tn : 2 * tn) * a.groups;
         const float* sw1 = GATE ? a.su + static_cast<int64_t>(tn) * a.groups
@@ -658,9 +699,13 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       if (lane == 0) mbar_arrive(used + 8 * (chunk & 1));
       ++chunk;
     };
-    for (int tile = pair, parity = 0; tile < tiles; tile += pairs, parity ^= 1) {
-      const int token = (tile % tiles_m) * 256 + rank * 128 + token_in;
-      const int tn = tile / tiles_m;
+    for (int unit = 0, parity = 0; unit < work.units; ++unit, parity ^= 1) {
+      int token, tn, half;
+      work.unit(unit, token, tn, half);
+      token += rank * 128 + token_in;
+      const bool whole = !kHalves || half < 0;
+      const int second = GATE ? 0 : whole ? part : half;  // which of the tile's weight blocks
+      const uint32_t columns = tmem + lanes + part * (GATE || !whole ? 64 : 128);
       const bool live = token < a.m;
       const int blocks = (a.n + 127) / 128;
       float acc[128];  // GATE: 64 columns of G, then the same of U
@@ -673,34 +718,41 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
         }
         const float* sc = scales + (chunk & 1) * kWideScales + (g % kWideChunk) * 128;
         const float sa = sc[token_in];
-        const float2 sw = *reinterpret_cast<const float2*>(scales + (chunk & 1) * kWideScales + kWideChunk * 128 +
-                                                           2 * (g % kWideChunk));
-        const float f0 = sa * (GATE || part == 0 ? sw.x : sw.y), f1 = sa * sw.y;
+        const float* sw = scales + (chunk & 1) * kWideScales + kWideChunk * 128 + 2 * (g % kWideChunk) + second;
+        const float f0 = sa * sw[0], f1 = GATE ? sa * sw[1] : f0;
         const int slot = i % kWideSlots;
         const int s = i % kWideStages;
         ok = ok && __all_sync(0xffffffffu, mbar_wait(done + 8 * s, (i / kWideStages) & 1, kGemmWaitCycles));
         if (!ok) continue;
         tc_fence_after();
-        // the next 32 columns are on their way from TMEM while these are added
-        const uint32_t src = tmem + lanes + slot * kWideCols + part * (GATE ? 64 : 128);
-        uint32_t p[2][32];
-        tmem_ld32(src, p[0]);
+        const uint32_t src = columns + slot * kWideCols;
+        // 32 columns at a time, the next ones on their way from TMEM while these are added
+        const auto add = [&](auto chunks) {
+          constexpr int kChunks = decltype(chunks)::value;
+          uint32_t p[2][32];
+          tmem_ld32(src, p[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_wait_ld();
-          if (c < 3) {
-            tmem_ld32(src + (GATE ? ((c + 1) >> 1) * 128 + ((c + 1) & 1) * 32 : (c + 1) * 32), p[(c + 1) & 1]);
-          } else {  // every column is in registers
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(freed + 8 * slot);
+          for (int c = 0; c < kChunks; ++c) {
+            tmem_wait_ld();
+            if (c + 1 < kChunks) {
+              tmem_ld32(src + (GATE ? ((c + 1) >> 1) * 128 + ((c + 1) & 1) * 32 : (c + 1) * 32), p[(c + 1) & 1]);
+            } else {  // every column is in registers
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(freed + 8 * slot);
+            }
+            const float2 f = GATE && c >= 2 ? make_float2(f1, f1) : make_float2(f0, f0);
+            float2* ac = reinterpret_cast<float2*>(acc + c * 32);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              ac[j] =
+                  fma2(make_float2(__uint_as_float(p[c & 1][2 * j]), __uint_as_float(p[c & 1][2 * j + 1])), f, ac[j]);
           }
-          const float2 f = GATE && c >= 2 ? make_float2(f1, f1) : make_float2(f0, f0);
-          float2* ac = reinterpret_cast<float2*>(acc + c * 32);
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            ac[j] = fma2(make_float2(__uint_as_float(p[c & 1][2 * j]), __uint_as_float(p[c & 1][2 * j + 1])), f, ac[j]);
-        }
+        };
+        if (whole)
+          add(std::integral_constant<int, 4>{});
+        else
+          add(std::integral_constant<int, 2>{});
       }
       next_chunk();
       if (!ok) {  // a wait that ran out leaves NaN, not a stale tile
@@ -734,9 +786,10 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       } else if (a.out_f32) {
 #pragma unroll
         for (int j = 0; j < 128; j += 32) {
-          const int col = tn * 256 + part * 128 + j;
+          if (j == 64 && !whole) break;
+          const int col = tn * 256 + (whole ? part * 128 : half * 128 + part * 64) + j;
           const uint4* w = reinterpret_cast<const uint4*>(acc + j);
-          if constexpr (!WORDS)
+          if constexpr (FORM != WideForm::kWords)
             store_tile<128>(&omap, col, token - lane, col < a.n && token - lane < a.m, w, turn + (j / 32 & 1) * kTurnBytes);
           else
             store_words<4>(static_cast<uint8_t*>(a.out) + (static_cast<int64_t>(token - lane) * a.n + col) * 4, a.n, false,
@@ -745,7 +798,8 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       } else {
 #pragma unroll
         for (int j = 0; j < 128; j += 64) {
-          const int col = tn * 256 + part * 128 + j;
+          if (j == 64 && !whole) break;
+          const int col = tn * 256 + (whole ? part * 128 : half * 128 + part * 64) + j;
           uint4 w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -753,7 +807,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
             w[i] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
                               pack_bf16x2(v[6], v[7]));
           }
-          if constexpr (!WORDS)
+          if constexpr (FORM != WideForm::kWords)
             store_tile<128>(&omap, col, token - lane, col < a.n && token - lane < a.m, w, turn + (j / 64) * kTurnBytes);
           else
             store_words<2>(static_cast<uint8_t*>(a.out) + (static_cast<int64_t>(token - lane) * a.n + col) * 2, a.n,
@@ -872,8 +926,8 @@ cudaError_t launch_gemm(const GemmCall& c, int splits, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<NT, GATE>, wmap, umap, amap, args);
 }
 
-template <bool GATE, bool WORDS>
-cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
+template <bool GATE, WideForm FORM>
+cudaError_t launch_wide(const GemmCall& c, int64_t tiles, cudaStream_t stream) {
   CUtensorMap wmap, umap, amap, omap = {};
   if (!encode_tiles(&wmap, c.w, c.args.n, c.k, c.ws, 128) || !encode_tiles(&amap, c.a, c.args.m, c.k, c.as, 128))
     return cudaErrorInvalidValue;
@@ -881,12 +935,11 @@ cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
   if (!encode_output(&omap, c.args, GATE)) return cudaErrorInvalidValue;
   if (GATE && !encode_tiles(&umap, c.u, c.args.n, c.k, c.us, 128)) return cudaErrorInvalidValue;
   const cudaError_t e =
-      cudaFuncSetAttribute(fp8_wide_kernel<GATE, WORDS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+      cudaFuncSetAttribute(fp8_wide_kernel<GATE, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
   if (e != cudaSuccess) return e;
-  const int columns = GATE ? 128 : 256;
-  const int64_t tiles = static_cast<int64_t>((c.args.m + 255) / 256) * ((c.args.n + columns - 1) / columns);
+  const int64_t units = FORM == WideForm::kHalves && tiles < kWidePairs ? 2 * tiles : tiles;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * static_cast<unsigned>(tiles < 74 ? tiles : 74));
+  cfg.gridDim = dim3(2 * static_cast<unsigned>(units < kWidePairs ? units : kWidePairs));
   cfg.blockDim = dim3(kWideThreads);
   cfg.dynamicSmemBytes = kWideSmem;
   cfg.stream = stream;
@@ -899,7 +952,7 @@ cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, fp8_wide_kernel<GATE, WORDS>, wmap, umap, amap, omap, c.args);
+  return cudaLaunchKernelEx(&cfg, fp8_wide_kernel<GATE, FORM>, wmap, umap, amap, omap, c.args);
 }
 
 // Which kernel, how many tokens per tile and how many blocks per tile: the least time by a
@@ -909,7 +962,8 @@ cudaError_t launch_wide(const GemmCall& c, cudaStream_t stream) {
 //   split kernel  start 2.0 + 0.012 c (GATE 0.5 more), 0.9 for every block an SM has to start
 //                 beyond its first; per column group 0.12 + 0.003 c, or the time in which all
 //                 blocks' operands come from L2 at 13 bytes/ps; summing up a split tile 0.3 + 0.02 c
-//   pair kernel   start 3.0; per wave of 74 tiles 0.40 per column group and 1.2 (GATE 2.0)
+//   pair kernel   start 3.0; per round of 74 tiles 0.40 per column group and 1.2 (GATE 2.0), a
+//                 last round of half tiles 0.31 and 1.0
 // Measured on either side of its borders: 512 x 960 x 960 4.3 us by 32 tokens a tile (64: 5.3,
 // pairs 7.3); 64 x 960 x 2560 3.9 by 16 tokens and 3 blocks a tile (one: 5.6; 64 tokens and 5
 // blocks: 4.8); 2048 x 1600 x 960 8.1 by pairs (64 tokens: 11.7).
@@ -918,12 +972,20 @@ struct GemmPlan {
   int splits;
 };
 
-GemmPlan make_gemm_plan(int m, int n, int groups, bool gate) {
+int64_t wide_tiles(const GemmArgs& a, bool gate) {
+  const int columns = gate ? 128 : 256;
+  return static_cast<int64_t>((a.m + 255) / 256) * ((a.n + columns - 1) / columns);
+}
+
+GemmPlan make_gemm_plan(const GemmArgs& a, bool gate) {
+  const int m = a.m, n = a.n, groups = a.groups;
   const int parts = gate ? 2 : 1;
-  const int wide_columns = gate ? 128 : 256;
-  const int64_t wide_tiles = static_cast<int64_t>((m + 255) / 256) * ((n + wide_columns - 1) / wide_columns);
+  const int64_t pair_tiles = wide_tiles(a, gate);
+  const bool halves = wide_form(a, pair_tiles, gate) == WideForm::kHalves;
   GemmPlan best{256, 1};
-  float least = 3.0f + static_cast<float>((wide_tiles + 73) / 74) * (groups * 0.40f + (gate ? 2.0f : 1.2f));
+  const float round = groups * 0.40f + (gate ? 2.0f : 1.2f);
+  float least = 3.0f + static_cast<float>(pair_tiles / kWidePairs) * round;
+  if (pair_tiles % kWidePairs > 0) least += halves ? groups * 0.31f + 1.0f : round;
   for (int nt = 16; nt <= (gate ? 32 : 64); nt *= 2) {
     const int64_t tiles = static_cast<int64_t>((n + kTileRows - 1) / kTileRows) * ((m + nt - 1) / nt);
     if (tiles > INT32_MAX / kMaxSplits || (m + nt - 1) / nt > 65535) continue;
@@ -952,16 +1014,26 @@ GemmPlan make_gemm_plan(int m, int n, int groups, bool gate) {
 }
 
 template <bool GATE>
+cudaError_t launch_pairs(const GemmCall& c, cudaStream_t stream) {
+  const int64_t tiles = wide_tiles(c.args, GATE);
+  if constexpr (!GATE) {
+    switch (wide_form(c.args, tiles, GATE)) {
+      case WideForm::kHalves: return launch_wide<GATE, WideForm::kHalves>(c, tiles, stream);
+      case WideForm::kWords: return launch_wide<GATE, WideForm::kWords>(c, tiles, stream);
+      default: break;
+    }
+  }
+  return launch_wide<GATE, WideForm::kWhole>(c, tiles, stream);
+}
+
+template <bool GATE>
 cudaError_t launch_planned(const GemmCall& c, cudaStream_t stream) {
-  const GemmPlan p = make_gemm_plan(c.args.m, c.args.n, c.args.groups, GATE);
+  const GemmPlan p = make_gemm_plan(c.args, GATE);
   switch (p.tokens) {
     case 16: return launch_gemm<16, GATE>(c, p.splits, stream);
     case 32: return launch_gemm<32, GATE>(c, p.splits, stream);
     case 64: return launch_gemm<GATE ? 32 : 64, GATE>(c, p.splits, stream);
-    default:
-      if (GATE || static_cast<int64_t>(c.args.n) * (c.args.out_f32 ? 4 : 2) % 16 == 0)
-        return launch_wide<GATE, false>(c, stream);
-      return launch_wide<GATE, !GATE>(c, stream);
+    default: return launch_pairs<GATE>(c, stream);
   }
 }
 

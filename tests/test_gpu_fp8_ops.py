@@ -350,6 +350,35 @@ def test_linear_by_pairs(cuda, m, n, k, dtype):
     assert torch.equal(G.fp8_linear(a, w, dtype), out)
 
 
+# The last round's tiles cut into halves of 128 columns: all of them, some, the most that are cut (37),
+# a second half of few columns and one of none.
+HALVES = [(512, 4096, 4096), (500, 4040, 1040), (2048, 2560, 400), (2100, 2200, 2064), (9467, 664, 144),
+          (9467, 608, 272)]
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('m,n,k', HALVES)
+def test_linear_by_halves(cuda, m, n, k, dtype):
+    gen = torch.Generator().manual_seed(m + n + k)
+    a, w = _rows(gen, m, k), _blocks(gen, n, k)
+    out = G.fp8_linear(a, w, dtype)
+    F.check_product(out, a, w)
+    assert torch.equal(G.fp8_linear(a, w, dtype), out)
+
+
+@pytest.mark.parametrize('m,n,block', [(2500, 4096, 30), (2500, 4096, 31), (500, 4040, 0), (500, 4040, 31)])
+def test_halves_keep_weight_blocks_apart(cuda, m, n, block):
+    """A NaN weight block reaches its own 128 columns: not the tile's other half, nor another group."""
+    gen = torch.Generator().manual_seed(block)
+    a, (wq, ws) = _rows(gen, m, 528), _blocks(gen, n, 528)
+    ref = G.fp8_linear(a, (wq, ws))
+    ws[block, 3] = float('nan')
+    out = G.fp8_linear(a, (wq, ws))
+    own = torch.arange(n, device='cuda') // 128 == block
+    assert torch.isnan(out[:, own]).all()
+    assert torch.equal(out[:, ~own], ref[:, ~own])
+
+
 @pytest.mark.parametrize('m,n,k', [(4096, 2560, 960), (3001, 2576, 272), (2304, 1040, 2064), (700, 6416, 400)])
 def test_gate_up_by_pairs(cuda, m, n, k):
     gen = torch.Generator().manual_seed(m + n + k)
