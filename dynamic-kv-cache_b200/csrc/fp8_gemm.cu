@@ -477,9 +477,12 @@ __device__ __forceinline__ void store_words(uint8_t* out, int64_t n, bool odd_st
 // How a pair kernel gives out its tiles and stores them: three kernels, because what the other
 // two need takes registers and clocks from the loop over the groups (one kernel for whole and half
 // tiles: 2048 x 4096 x 4096 34.8 us for 32.7; words in it: 4096 x 4097 x 4096 90 for 84).
-// kHalves: the last round's tiles, at most half as many as there are pairs, are cut into halves of
-// 128 weight rows. Products of 128 columns run at half rate (0.31 us a group for 0.40 of a whole
-// tile), but two pairs share a tile. GATE's tiles stay whole: a column group needs both halves.
+// kHalves: of at most three rounds, the last one's tiles (at most half as many as there are pairs)
+// are cut into halves of 128 weight rows. Products of 128 columns run at half rate (0.31 us a group
+// for 0.40 of a whole tile), but two pairs share a tile: 512 x 4096 x 4096 16.5 -> 15.5 us, 512 x
+// 960 x 2560 11.7 -> 10.5, after two whole rounds (2048 x 5120 x 960) 16.8 -> 16.1. After three they
+// cost more than they give (4096^3 62.2 -> 63.6), and GATE's tiles stay whole: a column group needs
+// both halves.
 // kWords: the output's rows do not start on 16 bytes.
 enum class WideForm { kWhole, kHalves, kWords };
 
@@ -487,7 +490,7 @@ WideForm wide_form(const GemmArgs& a, int64_t tiles, bool gate) {
   if (gate) return WideForm::kWhole;
   if (static_cast<int64_t>(a.n) * (a.out_f32 ? 4 : 2) % 16 != 0) return WideForm::kWords;
   const int64_t rest = tiles % kWidePairs;
-  return rest > 0 && 2 * rest <= kWidePairs ? WideForm::kHalves : WideForm::kWhole;
+  return rest > 0 && 2 * rest <= kWidePairs && tiles < 3 * kWidePairs ? WideForm::kHalves : WideForm::kWhole;
 }
 
 // The tiles of one pair of blocks, `pairs` apart, first token fastest.
@@ -963,9 +966,9 @@ cudaError_t launch_wide(const GemmCall& c, int64_t tiles, cudaStream_t stream) {
 //                 beyond its first; per column group 0.12 + 0.003 c, or the time in which all
 //                 blocks' operands come from L2 at 13 bytes/ps; summing up a split tile 0.3 + 0.02 c
 //   pair kernel   start 3.0; per round of 74 tiles 0.40 per column group and 1.2 (GATE 2.0), a
-//                 last round of half tiles 0.31 and 1.0
+//                 round of half tiles 0.31 and 1.0
 // Measured on either side of its borders: 512 x 960 x 960 4.3 us by 32 tokens a tile (64: 5.3,
-// pairs 7.3); 64 x 960 x 2560 3.9 by 16 tokens and 3 blocks a tile (one: 5.6; 64 tokens and 5
+// pairs 6.2); 64 x 960 x 2560 3.9 by 16 tokens and 3 blocks a tile (one: 5.6; 64 tokens and 5
 // blocks: 4.8); 2048 x 1600 x 960 8.1 by pairs (64 tokens: 11.7).
 struct GemmPlan {
   int tokens;  // per tile; 256: the pair kernel
