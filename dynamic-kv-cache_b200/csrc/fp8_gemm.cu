@@ -646,6 +646,11 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
           umma_commit_pair(done + 8 * s);
         }
       }
+      // The last arrivals from the other block are waited for as all others are: this block must
+      // not leave, and its shared memory go to another, while one is on its way.
+      if (ok)
+        for (int j = max(0, i - kWideSlots); j < i; ++j)
+          mbar_wait(freed + 8 * (j % kWideSlots), (j / kWideSlots) & 1, kGemmWaitCycles);
     }
     if (warp >= 10) {
       pdl_wait();

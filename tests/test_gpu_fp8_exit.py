@@ -1,0 +1,53 @@
+"""GPU checks of how the 8-bit products' blocks leave their SMs: nothing of one launch may reach
+the barriers, shared memory or TMEM of the next block there."""
+import pytest
+import torch
+
+import fp8_cases as F
+from src import gpu_ops as G
+
+pytestmark = pytest.mark.gpu
+
+
+def _rows(gen, m, k):
+    return F.torch_rows((torch.randn(m, k, generator=gen) * torch.exp(torch.randn(k, generator=gen))).cuda())
+
+
+def _blocks(gen, n, k):
+    return F.torch_blocks((torch.randn(n, k, generator=gen) * k ** -0.5).bfloat16().cuda())
+
+
+# Pair kernels of one to three column groups, whose blocks leave soonest after their last products:
+# one round of tiles, several, half tiles, rows stored by words, and gate/up.
+SHORT = [(512, 4096, 16), (512, 4096, 272), (4096, 4096, 128), (4096, 2560, 384), (2049, 5000, 144), (2305, 4098, 256)]
+
+
+def test_blocks_after_a_pair_kernel_find_their_own_barriers(cuda):
+    """Short pair kernels back to back and beside the split kernel's blocks on another stream, which
+    take over their SMs: every output is, bit for bit, what the same call gives alone."""
+    gen = torch.Generator().manual_seed(21)
+    calls = []
+    for m, n, k in SHORT:
+        a, w = _rows(gen, m, k), _blocks(gen, n, k)
+        calls.append(lambda a=a, w=w: (G.fp8_linear(a, w),))
+        if n % 16 == 0:
+            calls.append(lambda a=a, w=w: tuple(G.fp8_gate_up(a, w, w)))
+    small = [(_rows(gen, m, k), _blocks(gen, n, k)) for m, n, k in ((1, 1600, 960), (64, 960, 2560), (25, 2560, 960))]
+    calls_small = [lambda a=a, w=w: (G.fp8_linear(a, w, torch.float32),) for a, w in small]
+
+    def alone(call):
+        out = call()
+        torch.cuda.synchronize()
+        return out
+
+    bits = lambda out: [t.view(torch.uint8) for t in out]
+    expected, expected_small = [alone(c) for c in calls], [alone(c) for c in calls_small]
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for turn in range(20):
+        with torch.cuda.stream(streams[0]):
+            got = [c() for c in calls]
+        with torch.cuda.stream(streams[1]):
+            got_small = [c() for c in calls_small * 4]
+        torch.cuda.synchronize()
+        for out, ref in zip(got + got_small, expected + expected_small * 4):
+            assert all(torch.equal(x, y) for x, y in zip(bits(out), bits(ref))), turn
