@@ -115,6 +115,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[3 * T::kStages + 1];
   __shared__ uint32_t tmem_slot;
+  __shared__ int issued[2];  // groups whose copies and products were issued
   const uint32_t ring = (smem_addr(smem_raw) + 1023u) & ~1023u;
   uint8_t* const ring_ptr = smem_raw + (ring - smem_addr(smem_raw));
   // this block's own partial sums [part][token][weight row], in the ring once it is read
@@ -158,6 +159,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   }
   if (threadIdx.x == 0 && a.splits > 1) mbar_arrive_expect_tx(mailed, a.splits * T::kParts * mine * kTileRows * 4);
   __syncthreads();
+  bool ran_out = false;  // a wait for this block's products did
   if (a.splits > 1) cluster_arrive_release();  // this block has started: others may write to it
   pdl_wait();  // operands are the previous kernels' output
 
@@ -183,9 +185,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
           tile2d_g2s(dst + T::kParts * T::kWeightBytes, &amap, x, token0, full + 8 * s);
         }
       }
-      if (!ok)  // a wait that ran out: the copies in flight still target this block's memory
-        for (int j = max(0, i - a.stages); j < i; ++j)
-          mbar_wait(full + 8 * (j % a.stages), (j / a.stages) & 1, kGemmWaitCycles);
+      issued[0] = i;
     }
     __syncwarp();
   } else if (warp == 5) {
@@ -222,6 +222,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
           umma_commit(done + 8 * s);
         }
       }
+      issued[1] = i;
     }
     __syncwarp();
   } else if (warp < 4) {
@@ -271,18 +272,20 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       if (lane == 0) mbar_arrive(freed + 8 * slot);
       if (++slot == a.stages) slot = 0, phase ^= 1;
     }
-    // a wait that ran out leaves NaN, not a stale tile
+    // Where a wait ran out, copies may still arrive on these sums: they are not used or sent, and
+    // this block's tokens, and those of the blocks that wait for its sums, become NaN below.
 #pragma unroll
-    for (int j = 0; j < T::kCols; ++j) own[j * kTileRows + threadIdx.x] = ok ? acc[j] : __int_as_float(0x7fc00000);
+    for (int j = 0; j < T::kCols; ++j) own[j * kTileRows + threadIdx.x] = acc[j];
+    ran_out = !ok;
     if (a.splits > 1) {
       // Rank r adds up tokens [r * local, (r + 1) * local): one bulk copy per rank and part
       // (single stores to another block's shared memory were 5 times slower).
       fence_proxy_async_smem();
       cluster_wait_acquire();
-      named_bar_sync(3, 128);
+      ran_out = named_bar_or(3, 128, ran_out);
       const int to = threadIdx.x;
       const int n = min(local, live - to * local);
-      if (to < a.splits && n > 0) {
+      if (to < a.splits && n > 0 && !ran_out) {
 #pragma unroll
         for (int p = 0; p < T::kParts; ++p)
           bulk_s2s(dsmem_addr(mail + (rank * T::kParts + p) * local * kTileRows * 4, to),
@@ -294,18 +297,25 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   // TMEM goes back before this block waits for another one: what holds TMEM never depends
   // on a block that may still be waiting for some.
   tc_fence_before();
-  __syncthreads();
+  ran_out = __syncthreads_or(ran_out);
   if (warp == 5) {
+    if (ran_out && lane == 0) {  // copies and products that still use this block's memories end first
+      for (int j = max(0, issued[0] - a.stages); j < issued[0]; ++j)
+        mbar_wait(full + 8 * (j % a.stages), (j / a.stages) & 1, kGemmWaitCycles);
+      for (int j = max(0, issued[1] - a.stages); j < issued[1]; ++j)
+        mbar_wait(done + 8 * (j % a.stages), (j / a.stages) & 1, kGemmWaitCycles);
+    }
+    __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem_slot, T::kTmemCols);
   }
   const float* sums = own;
   int parts_apart = NT * kTileRows;
-  bool complete = true;
+  bool complete = !ran_out;
   if (a.splits > 1) {
     sums = reinterpret_cast<const float*>(ring_ptr + a.stages * T::kStageBytes);
     parts_apart = local * kTileRows;
-    if (mine > 0) complete = mbar_wait(mailed, 0, kGemmWaitCycles);
+    if (mine > 0) complete = mbar_wait(mailed, 0, kGemmWaitCycles);  // a block that ran out has sent nothing
   }
 
   // A warp per token, 4 weight rows (output columns) per lane: neighbouring ones where a row's

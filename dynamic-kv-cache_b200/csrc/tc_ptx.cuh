@@ -179,6 +179,22 @@ __device__ __forceinline__ void named_bar_sync(int id, int count) {
   asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(count) : "memory");
 }
 
+// The same, and whether any of the threads came with `flag`.
+__device__ __forceinline__ bool named_bar_or(int id, int count, bool flag) {
+  uint32_t any;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.u32 p, %3, 0;\n"
+      "bar.red.or.pred q, %1, %2, p;\n"
+      "selp.b32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(any)
+      : "r"(id), "r"(count), "r"(static_cast<uint32_t>(flag))
+      : "memory");
+  return any != 0;
+}
+
 // Counts this warp in at a hardware barrier that others wait on.
 __device__ __forceinline__ void named_bar_arrive(int id, int count) {
   asm volatile("bar.arrive %0, %1;\n" ::"r"(id), "r"(count) : "memory");

@@ -51,3 +51,18 @@ def test_blocks_after_a_pair_kernel_find_their_own_barriers(cuda):
         torch.cuda.synchronize()
         for out, ref in zip(got + got_small, expected + expected_small * 4):
             assert all(torch.equal(x, y) for x, y in zip(bits(out), bits(ref))), turn
+
+
+# Tiles of few tokens: fewer, as many and more column groups than stages (3 or 4), in one block and
+# split over clusters, down to clusters whose last blocks have no token to add up.
+FEW = [(1, 128, 16), (1, 40000, 144), (3, 130, 640), (40, 960, 400), (16, 128, 4096), (64, 30001, 528), (33, 20000, 1040)]
+
+
+@pytest.mark.parametrize('m,n,k', FEW)
+def test_split_kernel_ends_with_its_last_copies_and_products(cuda, m, n, k):
+    """Back to back launches, each against the 64-bit product, the last as the first."""
+    gen = torch.Generator().manual_seed(m + n + k)
+    a, w = _rows(gen, m, k), _blocks(gen, n, k)
+    out = [G.fp8_linear(a, w, torch.float32) for _ in range(20)]
+    F.check_product(out[0], a, w)
+    assert all(torch.equal(o, out[0]) for o in out[1:])
