@@ -618,7 +618,9 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
           }
         }
       }
-      if (!ok && rank == 0)  // a wait that ran out: the copies in flight still target shared memory
+      // Both blocks' last copies arrive before the pair leaves, also where a wait ran out here or
+      // in another warp (elsewhere the products have waited for them already).
+      if (rank == 0)
         for (int j = max(0, i - kWideStages); j < i; ++j)
           mbar_wait(full + 8 * (j % kWideStages), (j / kWideStages) & 1, kGemmWaitCycles);
     } else if (warp == 9 && rank == 1 && elect_one()) {
@@ -657,10 +659,14 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
         }
       }
       // The last arrivals from the other block are waited for as all others are: this block must
-      // not leave, and its shared memory go to another, while one is on its way.
-      if (ok)
-        for (int j = max(0, i - kWideSlots); j < i; ++j)
+      // not leave, and its shared memory go to another, while one is on its way. Where a wait ran
+      // out, the products in flight end before TMEM is freed.
+      for (int j = max(0, i - kWideSlots); j < i; ++j) {
+        if (ok)
           mbar_wait(freed + 8 * (j % kWideSlots), (j / kWideSlots) & 1, kGemmWaitCycles);
+        else
+          mbar_wait(done + 8 * (j % kWideStages), (j / kWideStages) & 1, kGemmWaitCycles);
+      }
     }
     if (warp >= 10) {
       pdl_wait();
