@@ -168,21 +168,34 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   // and a few additions is left in them (with addresses and descriptors made on the way, the
   // issuing took longer than the products).
   if (warp == 4) {
-    if (elect_one()) {
+    const bool issuer = elect_one();
+    const auto copy = [&](int s, int i) {
+      const uint32_t dst = ring + s * T::kStageBytes;
+      const int x = (group0 + i) * kFp8Group;
+      mbar_arrive_expect_tx(full + 8 * s, T::kStageBytes);
+      tile2d_g2s(dst, &wmap, x, tile * kTileRows, full + 8 * s);
+      if (GATE) tile2d_g2s(dst + T::kWeightBytes, &umap, x, tile * kTileRows, full + 8 * s);
+      tile2d_g2s(dst + T::kParts * T::kWeightBytes, &amap, x, token0, full + 8 * s);
+    };
+    if (issuer) {
+#pragma unroll
+      for (int s = 0; s < T::kStages; ++s) {
+        if (s >= count || s == a.stages) break;
+        copy(s, s);
+      }
+    }
+    __syncwarp();
+    named_bar_sync(4, 64);  // no wait of limited time before this block has its TMEM
+    if (issuer) {
       bool ok = true;
-      int i = 0;
-      for (uint32_t phase = 1; i < count && ok; phase ^= 1) {
+      int i = min(count, a.stages);
+      for (uint32_t phase = 0; i < count && ok; phase ^= 1) {
 #pragma unroll
         for (int s = 0; s < T::kStages; ++s, ++i) {
           if (i >= count || s == a.stages) break;
-          if (i >= a.stages) ok = mbar_wait(done + 8 * s, phase, kGemmWaitCycles);
+          ok = mbar_wait(done + 8 * s, phase, kGemmWaitCycles);
           if (!ok) break;
-          const uint32_t dst = ring + s * T::kStageBytes;
-          const int x = (group0 + i) * kFp8Group;
-          mbar_arrive_expect_tx(full + 8 * s, T::kStageBytes);
-          tile2d_g2s(dst, &wmap, x, tile * kTileRows, full + 8 * s);
-          if (GATE) tile2d_g2s(dst + T::kWeightBytes, &umap, x, tile * kTileRows, full + 8 * s);
-          tile2d_g2s(dst + T::kParts * T::kWeightBytes, &amap, x, token0, full + 8 * s);
+          copy(s, i);
         }
       }
       issued[0] = i;
@@ -195,6 +208,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
     tmem_relinquish();
     pdl_trigger();
     tc_fence_before();
+    named_bar_arrive(4, 64);
     named_bar_arrive(2, 160);  // the products need not wait for the scales
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
@@ -293,7 +307,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       }
     }
   }
-  if (a.splits > 1 && warp >= 4) cluster_wait_acquire();
+  if (a.splits > 1) {
+    if (warp >= 4) cluster_wait_acquire();
+    cluster_arrive_relaxed();  // this block has its TMEM, and its sums are on their way
+  }
   // TMEM goes back before this block waits for another one: what holds TMEM never depends
   // on a block that may still be waiting for some.
   tc_fence_before();
@@ -315,7 +332,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   if (a.splits > 1) {
     sums = reinterpret_cast<const float*>(ring_ptr + a.stages * T::kStageBytes);
     parts_apart = local * kTileRows;
-    if (mine > 0) complete = mbar_wait(mailed, 0, kGemmWaitCycles);  // a block that ran out has sent nothing
+    // The time counts from when every block had its TMEM, which another stream's kernel may hold for
+    // long; where all goes well that is past before the sums are here. A block that ran out sends nothing.
+    if (mine > 0) complete = mbar_wait(mailed, 0, kGemmWaitCycles);
+    __syncwarp();
+    cluster_wait_acquire();
+    if (!complete) complete = mbar_wait(mailed, 0, kGemmWaitCycles);
   }
 
   // A warp per token, 4 weight rows (output columns) per lane: neighbouring ones where a row's
@@ -587,7 +609,10 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       tc_fence_after();
       pdl_trigger();  // after both blocks' allocation
     }
-    if (warp == 8 && elect_one()) {
+    // No wait of limited time begins before both blocks have their TMEM, which another stream's
+    // kernel may hold for long: each role waits for the rendezvous before its first.
+    if (warp == 8) {
+      const bool issuer = elect_one();
       const uint32_t full0 = dsmem_addr(full, 0);
       const CUtensorMap* const rows = GATE && rank == 1 ? &umap : &wmap;
       int unit = 0, x = 0, token0, row0;
@@ -597,32 +622,46 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
         token0 += rank * 128;
         row0 = GATE ? tn * 128 : half < 0 ? tn * 256 + rank * 128 : tn * 256 + half * 128 + rank * 64;
       };
+      const auto copy = [&](int s) {
+        const uint32_t dst = ring + s * kWideStageBytes;
+        if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, 2 * kWideStageBytes);
+        tile2d_g2s_pair(dst, &amap, x, token0, full0 + 8 * s);
+        tile2d_g2s_pair(dst + kWideHalf, rows, x, row0, full0 + 8 * s);
+        x += kFp8Group;
+        if (x >= a.groups * kFp8Group) {
+          x = 0;
+          next();
+        }
+      };
       next();
-      pdl_wait();
-      bool ok = true;
-      int i = 0;
-      for (uint32_t phase = 1; i < total && ok; phase ^= 1) {
+      if (issuer) {
+        pdl_wait();
 #pragma unroll
-        for (int s = 0; s < kWideStages; ++s, ++i) {
-          if (i >= total) break;
-          if (i >= kWideStages) ok = mbar_wait(done + 8 * s, phase, kGemmWaitCycles);
-          if (!ok) break;
-          const uint32_t dst = ring + s * kWideStageBytes;
-          if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, 2 * kWideStageBytes);
-          tile2d_g2s_pair(dst, &amap, x, token0, full0 + 8 * s);
-          tile2d_g2s_pair(dst + kWideHalf, rows, x, row0, full0 + 8 * s);
-          x += kFp8Group;
-          if (x >= a.groups * kFp8Group) {
-            x = 0;
-            next();
-          }
+        for (int s = 0; s < kWideStages; ++s) {
+          if (s >= total) break;
+          copy(s);
         }
       }
-      // Both blocks' last copies arrive before the pair leaves, also where a wait ran out here or
-      // in another warp (elsewhere the products have waited for them already).
-      if (rank == 0)
-        for (int j = max(0, i - kWideStages); j < i; ++j)
-          mbar_wait(full + 8 * (j % kWideStages), (j / kWideStages) & 1, kGemmWaitCycles);
+      __syncwarp();
+      cluster_wait_acquire();
+      if (issuer) {
+        bool ok = true;
+        int i = min(total, kWideStages);
+        for (uint32_t phase = 0; i < total && ok; phase ^= 1) {
+#pragma unroll
+          for (int s = 0; s < kWideStages; ++s, ++i) {
+            if (i >= total) break;
+            ok = mbar_wait(done + 8 * s, phase, kGemmWaitCycles);
+            if (!ok) break;
+            copy(s);
+          }
+        }
+        // Both blocks' last copies arrive before the pair leaves, also where a wait ran out here or
+        // in another warp (elsewhere the products have waited for them already).
+        if (rank == 0)
+          for (int j = max(0, i - kWideStages); j < i; ++j)
+            mbar_wait(full + 8 * (j % kWideStages), (j / kWideStages) & 1, kGemmWaitCycles);
+      }
     } else if (warp == 9 && rank == 1 && elect_one()) {
       // rank 1's eight warps reach rank 0 as one arrival
       const uint32_t freed0 = dsmem_addr(freed, 0);
@@ -675,7 +714,7 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
       // over in shared memory, it is one conflict-free load.
       const int t = threadIdx.x - 32 * 10;
       int c = 0;
-      bool ok = true;
+      bool ok = true, met = false;
       for (int unit = 0; unit < work.units && ok; ++unit) {
         int token0, tn, half;
         work.unit(unit, token0, tn, half);
@@ -686,6 +725,11 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
                                 : a.sw + static_cast<int64_t>(min(2 * tn + 1, (a.n + 127) / 128 - 1)) * a.groups;
         for (int g0 = 0; g0 < a.groups; g0 += kWideChunk, ++c) {
           const int n = min(kWideChunk, a.groups - g0);
+          if (c == 2) {
+            __syncwarp();
+            cluster_wait_acquire();
+            met = true;
+          }
           if (c >= 2 && !mbar_wait(used + 8 * (c & 1), ((c >> 1) + 1) & 1, kGemmWaitCycles)) {
             ok = false;
             break;
@@ -702,14 +746,16 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
           cp_async_mbar_arrive(staged + 8 * (c & 1));
         }
       }
+      __syncwarp();
+      if (!met) cluster_wait_acquire();  // no third chunk
     }
     __syncwarp();
-    if (warp != 9) cluster_wait_acquire();
   } else {
     regs_take<216>();
     cluster_arrive_relaxed();
     pdl_wait();
     named_bar_sync(2, 288);
+    cluster_wait_acquire();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     const int part = warp >> 2;
@@ -843,7 +889,6 @@ fp8_wide_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
   }
   // the other block's copies, arrivals and products are done with this one (no memory to order:
   // a release would wait for this block's stores)
-  if (warp < 8) cluster_wait_acquire();
   tc_fence_before();
   cluster_arrive_relaxed();
   cluster_wait_acquire();

@@ -66,3 +66,36 @@ def test_split_kernel_ends_with_its_last_copies_and_products(cuda, m, n, k):
     out = [G.fp8_linear(a, w, torch.float32) for _ in range(20)]
     F.check_product(out[0], a, w)
     assert all(torch.equal(o, out[0]) for o in out[1:])
+
+
+def test_products_of_every_kind_at_once_share_the_tensor_memory(cuda):
+    """Three streams of products whose blocks share SMs and want more accumulator columns together
+    than an SM has, beside the attention on a fourth: the ones that have to wait for columns, or for
+    a block of their cluster that does, give what they give alone."""
+    from src.gpu_cache import GPUCache
+    gen = torch.Generator().manual_seed(5)
+    past, heads, group, nq = 4096, 5, 3, 64
+    cache = GPUCache(None, layers=1, heads=heads, max_tokens=past + nq)
+    kv = torch.randn(1, heads, past, 64, generator=gen).bfloat16().cuda()
+    cache.select(8, 0)
+    cache.append(kv, kv, 0)
+    q = torch.randn(1, heads * group, nq, 64, generator=gen).bfloat16().cuda()
+    k = torch.randn(1, heads, nq, 64, generator=gen).bfloat16().cuda()
+    attend = lambda: cache.attend(q, k, k, 0, past)
+    linear = lambda m, n, k: (lambda a=_rows(gen, m, k), w=_blocks(gen, n, k): G.fp8_linear(a, w))
+    gate_up = lambda m, n, k: (lambda a=_rows(gen, m, k), w=_blocks(gen, n, k): G.fp8_gate_up(a, w, w).q.view(torch.uint8))
+    work = [[linear(64, 30001, 1040), linear(64, 960, 2560), linear(512, 1600, 960)],
+            [gate_up(256, 2560, 960), gate_up(25, 2560, 960), gate_up(1, 8192, 528)],
+            [linear(1, 1600, 960), linear(2048, 4096, 528), linear(25, 49280, 144)], [attend]]
+    alone = [[call() for call in calls] for calls in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    for _ in range(10):
+        got = [[] for _ in work]
+        for _ in range(4):
+            for s, calls, out in zip(streams, work, got):
+                with torch.cuda.stream(s):
+                    out.extend(call() for call in calls)
+        torch.cuda.synchronize()
+        for out, ref in zip(got, alone):
+            assert all(torch.equal(a, b) for a, b in zip(out, ref * 4))
