@@ -7,6 +7,7 @@
 // cost is paid on every layer of every frame.
 #include <torch/extension.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -183,10 +184,13 @@ constexpr int64_t kGroup = 128;
 
 int64_t groups_of(int64_t width) { return (width + kGroup - 1) / kGroup; }
 
-// The operators have no backward pass: a call that autograd would have to follow is refused.
+// The operators have no derivative: an operand (rows, weights, codes or scales) that autograd would
+// have to follow is refused, backward (requires_grad) as forward (a dual tensor's tangent).
 void no_grad(const at::Tensor& x, const char* what) {
   if (x.requires_grad() && at::GradMode::is_enabled())
     throw pybind11::value_error(std::string(what) + " has no backward pass (call it under torch.no_grad())");
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && x._fw_grad(0).defined())
+    throw pybind11::value_error(std::string(what) + " has no derivative: the tangent of an operand would be lost");
 }
 
 // bf16 [..., width] as rows the kernels can load 16 bytes at a time; `stride` receives
@@ -210,6 +214,7 @@ at::Tensor bf16_rows(const at::Tensor& x, const char* what, int64_t* stride) {
 at::Tensor e4m3_rows(const at::Tensor& q, const char* what, int64_t* stride) {
   if (!q.is_cuda() || q.scalar_type() != at::kFloat8_e4m3fn || q.dim() < 1)
     throw pybind11::value_error(std::string(what) + " takes CUDA float8_e4m3fn codes");
+  no_grad(q, what);
   const int64_t width = q.size(-1);
   if (q.dim() == 2 && q.size(0) > 0 && q.stride(1) == 1 && q.stride(0) >= width && q.stride(0) % 16 == 0 &&
       (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15u) == 0) {
@@ -227,6 +232,7 @@ at::Tensor row_scales(const at::Tensor& s, const at::Tensor& q, const char* what
             s.size(-1) == groups_of(q.size(-1));
   for (int64_t d = 0; ok && d + 1 < q.dim(); ++d) ok = s.size(d) == q.size(d);
   if (!ok) throw pybind11::value_error(std::string(what) + ": rows need fp32 scales [..., ceil(width / 128)] on their device");
+  no_grad(s, what);
   return s.contiguous();
 }
 
@@ -236,6 +242,7 @@ at::Tensor block_scales(const at::Tensor& s, const at::Tensor& q, const char* wh
       s.size(0) != groups_of(q.size(0)) || s.size(1) != groups_of(q.size(1)))
     throw pybind11::value_error(std::string(what) +
                                 ": weights are [n, k] with fp32 scales [ceil(n / 128), ceil(k / 128)] on their device");
+  no_grad(s, what);
   return s.contiguous();
 }
 
