@@ -39,6 +39,7 @@ cudaError_t launch_fp8_linear(const void* a, const float* sa, const void* w, con
 cudaError_t launch_fp8_gate_up(const void* a, const float* sa, const void* gate, const float* sg, const void* up,
                                const float* su, void* out, float* out_scale, int m, int n, int k, int64_t as,
                                int64_t gs, int64_t us, cudaStream_t stream);
+void fp8_plan(int m, int n, int k, int out_bits, int* plan);
 cudaError_t launch_pack_many(const void* k, const void* v, const dkv_pack_target* targets, bool on_device, int count,
                              int64_t kh, int64_t kt, int64_t vh, int64_t vt, int64_t kc, int64_t vc, int layer, int n,
                              int heads, int blocks, cudaStream_t stream);
@@ -668,13 +669,19 @@ int dkv_add_rms_norm_fp8(const void* x, const void* y, void* x_out, void* q, flo
                                 "add_rms_norm_fp8 launch"));
 }
 
+// Rows and weight rows of the 8-bit products.
+static int check_fp8_rows(const char* what, int64_t m, int32_t n) {
+  if (m < 0 || m > (1 << 21)) return fail(DKV_EINVAL, "%s: 0 to 2^21 rows", what);
+  if (n <= 0 || n > (1 << 24)) return fail(DKV_EINVAL, "%s: 1 to 2^24 weight rows", what);
+  return DKV_OK;
+}
+
 int dkv_fp8_linear(const void* a, const float* a_scale, const void* w, const float* w_scale, void* out,
                    int32_t out_bits, int64_t m, int32_t n, int32_t k, int64_t as, int64_t ws, void* stream) {
   int rc = check_fp8_width("fp8_linear", k);
   if (rc) return rc;
   if (out_bits != 16 && out_bits != 32) return fail(DKV_EINVAL, "fp8_linear: out is bf16 (16) or fp32 (32)");
-  if (m < 0 || m > (1 << 21)) return fail(DKV_EINVAL, "fp8_linear: 0 to 2^21 rows");
-  if (n <= 0 || n > (1 << 24)) return fail(DKV_EINVAL, "fp8_linear: 1 to 2^24 weight rows");
+  if ((rc = check_fp8_rows("fp8_linear", m, n))) return rc;
   if (m == 0) return ok();
   if (!a || !a_scale || !w || !w_scale || !out) return fail(DKV_EINVAL, "fp8_linear: null pointer");
   if (!aligned16(a) || !aligned16(w) || !aligned16(out) || !aligned4(a_scale) || !aligned4(w_scale))
@@ -694,7 +701,7 @@ int dkv_fp8_gate_up(const void* a, const float* a_scale, const void* gate, const
   int rc = check_fp8_width("fp8_gate_up", k);
   if (rc) return rc;
   if ((rc = check_fp8_width("fp8_gate_up output", n))) return rc;
-  if (m < 0 || m > (1 << 21)) return fail(DKV_EINVAL, "fp8_gate_up: 0 to 2^21 rows");
+  if ((rc = check_fp8_rows("fp8_gate_up", m, n))) return rc;
   if (m == 0) return ok();
   if (!a || !a_scale || !gate || !gate_scale || !up || !up_scale || !q || !scale)
     return fail(DKV_EINVAL, "fp8_gate_up: null pointer");
@@ -708,6 +715,19 @@ int dkv_fp8_gate_up(const void* a, const float* a_scale, const void* gate, const
                                                         static_cast<int>(m), n, k, as, gs, us,
                                                         static_cast<cudaStream_t>(stream)),
                                 "fp8_gate_up launch"));
+}
+
+int dkv_fp8_plan(int64_t m, int32_t n, int32_t k, int32_t out_bits, int32_t* plan) {
+  int rc = check_fp8_width("fp8_plan", k);
+  if (rc) return rc;
+  if (out_bits != 8 && out_bits != 16 && out_bits != 32)
+    return fail(DKV_EINVAL, "fp8_plan: out is e4m3 of gate/up (8), bf16 (16) or fp32 (32)");
+  if (out_bits == 8 && (rc = check_fp8_width("fp8_plan output", n))) return rc;
+  if ((rc = check_fp8_rows("fp8_plan", m, n))) return rc;
+  if (m == 0) return fail(DKV_EINVAL, "fp8_plan: no rows, no launch");
+  if (!plan) return fail(DKV_EINVAL, "fp8_plan: null pointer");
+  dkv::fp8_plan(static_cast<int>(m), n, k, out_bits, plan);
+  return ok();
 }
 
 }  // extern "C"

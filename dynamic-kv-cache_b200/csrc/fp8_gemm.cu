@@ -957,6 +957,13 @@ struct GemmCall {
   GemmArgs args;
 };
 
+// Operand stages of the split kernel: one more where blocks have an SM to themselves; two or three
+// share it otherwise.
+int gemm_stages(const GemmArgs& a, int tokens, int splits) {
+  const int64_t blocks = static_cast<int64_t>((a.n + kTileRows - 1) / kTileRows) * splits * ((a.m + tokens - 1) / tokens);
+  return blocks <= 148 ? 4 : 3;
+}
+
 template <int NT, bool GATE>
 cudaError_t launch_gemm(const GemmCall& c, int splits, cudaStream_t stream) {
   using T = GemmTile<NT, GATE>;
@@ -968,9 +975,8 @@ cudaError_t launch_gemm(const GemmCall& c, int splits, cudaStream_t stream) {
   GemmArgs args = c.args;
   args.splits = splits;
   const int per = (args.groups + splits - 1) / splits;
-  // one more stage where blocks have an SM to themselves; two or three share it otherwise
-  const int64_t blocks = static_cast<int64_t>((args.n + kTileRows - 1) / kTileRows) * splits * ((args.m + NT - 1) / NT);
-  args.stages = blocks <= 148 ? T::kStages : 3;
+  args.stages = gemm_stages(args, NT, splits);
+  static_assert(T::kStages == 4, "gemm_stages");
   const int smem = T::smem(args.stages, splits, per);
   // the same limit for every call: threads that launch other shapes at the same time set it too
   cudaError_t e =
@@ -1107,6 +1113,18 @@ cudaError_t launch_planned(const GemmCall& c, cudaStream_t stream) {
 }
 
 }  // namespace
+
+// out_bits 8: gate/up. plan: tokens per tile (256: pairs), blocks per tile, stages, the pair kernel's form.
+void fp8_plan(int m, int n, int k, int out_bits, int* plan) {
+  const bool gate = out_bits == 8;
+  const GemmArgs a{nullptr, nullptr, nullptr, nullptr, nullptr, m, n, (k + kFp8Group - 1) / kFp8Group, 1, 0, out_bits == 32};
+  const GemmPlan p = make_gemm_plan(a, gate);
+  const bool pairs = p.tokens == 256;
+  plan[0] = p.tokens;
+  plan[1] = pairs ? 1 : p.splits;
+  plan[2] = pairs ? kWideStages : gemm_stages(a, p.tokens, p.splits);
+  plan[3] = pairs ? static_cast<int>(wide_form(a, wide_tiles(a, gate), gate)) : 0;
+}
 
 cudaError_t launch_fp8_linear(const void* a, const float* sa, const void* w, const float* sw, void* out, int out_f32,
                               int m, int n, int k, int64_t as, int64_t ws, cudaStream_t stream) {

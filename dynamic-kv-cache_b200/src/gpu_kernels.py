@@ -89,6 +89,7 @@ def _load():
         'dkv_add_rms_norm_fp8': ([P, P, P, P, P, P, I64, I32, I64, I64, I64, ctypes.c_float, P], ctypes.c_int),
         'dkv_fp8_linear': ([P, P, P, P, P, I32, I64, I32, I32, I64, I64, P], ctypes.c_int),
         'dkv_fp8_gate_up': ([P, P, P, P, P, P, P, P, I64, I32, I32, I64, I64, I64, P], ctypes.c_int),
+        'dkv_fp8_plan': ([I64, I32, I32, I32, P], ctypes.c_int),
         'dkv_append_attention_many_device': ([P, P, P, P, P, I32, I32, P, I64, I64, I64, I64, I64, I64, I64, I64, I64,
                                               I64, I32, I32, I32, I32, I32, I32, P, SZ, P], ctypes.c_int),
         'dkv_pool_granularity': ([I32], U64),
@@ -118,7 +119,7 @@ EXPORTS = ('dkv_version', 'dkv_last_error', 'dkv_pack_rows', 'dkv_packed_attenti
            'dkv_packed_attention_many', 'dkv_packed_attention_many_workspace', 'dkv_pack_rows_many_device',
            'dkv_packed_attention_many_device', 'dkv_append_attention', 'dkv_append_attention_many_device',
            'dkv_rotary', 'dkv_silu_mul', 'dkv_fp8_quantize', 'dkv_fp8_quantize_weight', 'dkv_add_rms_norm_fp8',
-           'dkv_fp8_linear', 'dkv_fp8_gate_up', 'dkv_pool_granularity', 'dkv_pool_create', 'dkv_pool_map',
+           'dkv_fp8_linear', 'dkv_fp8_gate_up', 'dkv_fp8_plan', 'dkv_pool_granularity', 'dkv_pool_create', 'dkv_pool_map',
            'dkv_pool_base', 'dkv_pool_mapped_bytes', 'dkv_pool_reserved_bytes', 'dkv_pool_destroy')
 
 

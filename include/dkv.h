@@ -500,6 +500,15 @@ int dkv_fp8_gate_up(const void* a, const float* a_scale, const void* gate, const
                     const float* up_scale, void* q, float* scale, int64_t m, int32_t n, int32_t k, int64_t as,
                     int64_t gs, int64_t us, void* stream);
 
+/*
+ * How dkv_fp8_linear (out_bits 16 or 32) or dkv_fp8_gate_up (8) would run a product of m
+ * rows, n weight rows and k columns; decided by these sizes alone, on the host. plan[0]:
+ * tokens per tile (16, 32 or 64; 256: pairs of blocks), [1]: blocks that share a tile's
+ * column groups, [2]: operand stages of a block, [3]: the pairs' form (0 whole tiles, 1
+ * the last ones cut into halves, 2 rows stored by words).
+ */
+int dkv_fp8_plan(int64_t m, int32_t n, int32_t k, int32_t out_bits, int32_t* plan);
+
 #ifdef __cplusplus
 }
 #endif
