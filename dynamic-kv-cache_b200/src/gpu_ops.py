@@ -49,7 +49,8 @@ def activation_product(gate, up):
 # -- 8-bit projections (dkv_fp8_*; not in the reference) ---------------------------
 # e4m3 codes with fp32 scales: activations one scale per row and group of 128
 # columns, weights one per block of 128 x 128 (scale = amax / 448, include/dkv.h).
-# CUDA only, widths multiples of 16, no backward pass. Sums stay in fp32 and each
+# CUDA only, widths multiples of 16 up to 16384, products of up to 2^21 rows, no derivative
+# (an operand that autograd would have to follow is refused). Sums stay in fp32 and each
 # result is rounded once; a NaN or infinity in a group makes its products NaN.
 
 class Fp8(NamedTuple):

@@ -457,6 +457,14 @@ int dkv_add_rms_norm(const void* x, const void* y, void* x_out, void* h_out, con
  * given; row strides of 8-bit matrices are in bytes, multiples of 16. Input and output
  * tensors of one call must not overlap. 16-byte aligned tensors (scales: 4). Nothing
  * here needs a workspace; every entry point may be captured into a CUDA graph.
+ * Limits (else DKV_EINVAL): products take up to 2^21 rows, weights have up to 2^24 rows
+ * (gate and up 16384); dkv_fp8_quantize and dkv_add_rms_norm_fp8 take more rows than that
+ * (2^31 - 1 in all, for the former over its column groups), which a product reads in parts.
+ * A product multiplies a row's and a block's scale first, in fp32: two scales whose product
+ * reaches 2^128 make the group infinite or NaN, and one below 2^-126 loses digits.
+ * These calls have no status word: a product whose pipeline makes no progress for ~0.2 s
+ * after it has its tensor memory (no healthy wait comes near it) gives NaN in the tiles
+ * concerned, although the call returned DKV_OK.
  */
 
 /* bf16 rows to e4m3 rows: x [rows, width] (row stride xs elements, a multiple of 8) ->
