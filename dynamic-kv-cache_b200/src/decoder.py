@@ -14,6 +14,7 @@ projections='fp8' (CUDA; not in the reference) runs the projections in 8 bits: t
 joined weights are e4m3 blocks (half the bytes a step has to stream), the norms write
 the e4m3 rows the projections read, and gate, up, SiLU and their product are one
 launch. Residual stream, attention, norms' sums, embeddings and logits stay as they are.
+Its load_state_dict takes a bf16 decoder's state too and quantises the projections.
 """
 from dataclasses import dataclass
 
@@ -122,6 +123,7 @@ class Decoder(torch.nn.Module):
         self.qkv = per_layer(qkv_out, cfg.hidden)
         self.o = per_layer(cfg.hidden, cfg.q_heads * cfg.head_dim)
         if self.fp8:  # gate and up apart: each one's blocks begin at its own first row
+            self.register_load_state_dict_pre_hook(Decoder._quantise_state)
             self.gate, self.up = torch.nn.ModuleList(), torch.nn.ModuleList()
             for _ in range(cfg.layers):
                 gate, up = w(2 * cfg.intermediate, cfg.hidden).chunk(2)
@@ -134,6 +136,21 @@ class Decoder(torch.nn.Module):
         self.norm_attn = torch.nn.ParameterList([ones() for _ in range(cfg.layers)])
         self.norm_mlp = torch.nn.ParameterList([ones() for _ in range(cfg.layers)])
         self.norm_out = ones()
+
+    def _quantise_state(self, state, prefix, *_):
+        """Projections in `state` that a bf16 decoder of this shape holds, as this one's 8-bit blocks."""
+        for name, parts in (('qkv', ('qkv',)), ('o', ('o',)), ('gate_up', ('gate', 'up')), ('down', ('down',))):
+            for layer in range(self.cfg.layers):
+                held = [getattr(self, part)[layer].q for part in parts]
+                w = state.get(f'{prefix}{name}.{layer}')
+                if w is None:
+                    continue
+                if w.shape != (sum(q.shape[0] for q in held), held[0].shape[1]):  # loading says which do not fit
+                    continue
+                del state[f'{prefix}{name}.{layer}']
+                for part, q, rows in zip(parts, held, w.detach().split([q.shape[0] for q in held])):
+                    blocks = fp8_quantize_weight(rows.to(q.device, torch.bfloat16))
+                    state[f'{prefix}{part}.{layer}.q'], state[f'{prefix}{part}.{layer}.scale'] = blocks
 
     def rms(self, x, weight):
         return cuda_rms(x, weight, self.cfg.rms_eps)
