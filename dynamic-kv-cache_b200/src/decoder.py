@@ -92,6 +92,14 @@ class Fp8Weight(torch.nn.Module):
         self.register_buffer('q', q)
         self.register_buffer('scale', scale)
 
+    def _apply(self, fn, recurse=True):
+        """Moves with its module; casts (to(torch.bfloat16), float()) are for the other weights."""
+        q, scale = self.q, self.scale
+        super()._apply(fn, recurse)
+        if (self.q.dtype, self.scale.dtype) != (q.dtype, scale.dtype):
+            self.q, self.scale = q.to(self.q.device), scale.to(self.scale.device)
+        return self
+
     @property
     def blocks(self):
         return Fp8(self.q, self.scale)

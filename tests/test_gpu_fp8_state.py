@@ -52,3 +52,16 @@ def test_a_state_under_a_prefix_and_one_that_does_not_fit(cuda):
     state['down.0'] = Decoder(SMALL, seed=0).state_dict()['down.0']
     model.load_state_dict(state)
     assert torch.equal(_logits(model), before)
+
+
+def test_moves_and_casts_leave_codes_and_scales_as_they_are(cuda):
+    """model.to(torch.bfloat16), model.float() and the like are for the other weights."""
+    model = Decoder(SMALL, projections='fp8')
+    before, held = _logits(model), {k: v.clone() for k, v in model.state_dict().items()}
+    for cast in (lambda: model.to(torch.bfloat16), lambda: model.bfloat16(), lambda: model.to('cuda', torch.bfloat16),
+                 lambda: model.cpu().cuda(), lambda: model.to(torch.float32).to(torch.bfloat16)):
+        cast()
+        now = model.state_dict()
+        assert all(now[k].dtype == held[k].dtype and now[k].device == held[k].device for k in held)
+        assert all(torch.equal(now[k].float(), held[k].float()) for k in held)
+        assert torch.equal(_logits(model), before)
