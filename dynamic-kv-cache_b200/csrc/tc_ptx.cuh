@@ -138,9 +138,6 @@ __device__ __forceinline__ void bulk_wait_read() {
   asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory");
 }
 
-// ... until all groups are written.
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
-
 // tile2d_g2s from a block of a CTA pair: `bar` may lie in the other block (dsmem_addr).
 __device__ __forceinline__ void tile2d_g2s_pair(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
   asm volatile(
