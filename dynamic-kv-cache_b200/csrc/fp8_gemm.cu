@@ -15,13 +15,13 @@
 // alone would leave SMs idle; their partial sums cross by bulk copies between the SMs' shared
 // memories and are added in rank order. Small calls are bound by latency, a chain of the
 // previous kernel's end (~1 us), the first copies (~0.5), the products (~0.2), the scaling
-// (0.1 to 0.2 a group) and the sums and stores (0.3 to 0.8): 1 x 1600 x 960 2.75 us, 64 x 960 x
-// 2560 3.6, 333 x 1001 x 1040 5.4; many weight rows by memory: 25 x 49280 x 960 11.4 us, 4.6 of
-// 6.6 TB/s.
+// (0.1 to 0.2 a group) and the sums and stores (0.3 to 0.8): 1 x 1600 x 960 2.7 us, 64 x 960 x
+// 2560 3.6, 333 x 1001 x 1040 5.2; many weight rows by memory: 25 x 49280 x 960 11.1 us, 4.7 of
+// 6.6 TB/s. (Times here: one launch of a replayed graph of 20, unless said.)
 //
-// fp8_wide_kernel (many tokens) is described below: 4096^3 64 us, 2.15 PFLOP/s, 65 % of twice
-// the measured bf16 rate (a plain library product of these e4m3 matrices, without block scales:
-// 49.5 us), bound by the round trip of an accumulator between the tensor cores and the threads
+// fp8_wide_kernel (many tokens) is described below: 4096^3 64.5 us (76 in a long run of calls, under
+// the power cap), 2.13 PFLOP/s, 65 % of twice the measured bf16 rate (a plain library product of
+// these e4m3 matrices, without block scales: 49.5 us), bound by the round trip of an accumulator between the tensor cores and the threads
 // that scale it, and by 3.46 tiles per pair of SMs taking the time of 4.
 //
 // GATE computes two products with the same rows, G and U, and writes silu(g) * u as e4m3
@@ -418,9 +418,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
 // need 48, and L2 gives an SM ~65 bytes per clock). Two accumulators of 256 columns fill
 // TMEM: while the tensor cores sum one group into one (512 clocks at their rate), the eight
 // epilogue warps scale and add the other. An accumulator's round (products, completion,
-// reading, release) takes ~1400 clocks, so two of them make a group ~700. Four accumulators of
-// 128 columns lost (products of 128 columns run at half rate: 96 us for 4096^3 against 67), as
-// did sixteen epilogue warps of 64 columns (72.6 against 70.3).
+// reading, release) takes ~1400 clocks, so two of them make a group ~700. In the builds that tried
+// them, four accumulators of 128 columns lost (products of 128 columns run at half rate: 96 us for
+// 4096^3 against 67), as did sixteen epilogue warps of 64 columns (72.6 against 70.3).
 // A thread owns one token and 128 columns; a group costs it a scale product and 64 packed FMAs.
 // The grid is persistent (one pair per two SMs): a tile's way out overlaps the next tile's first
 // groups. GATE gives the pair's first block the gate rows and the second the up rows of the
@@ -507,14 +507,15 @@ __device__ __forceinline__ void store_words(uint8_t* out, int64_t n, bool odd_st
 }
 
 // How a pair kernel gives out its tiles and stores them: three kernels, because what the other
-// two need takes registers and clocks from the loop over the groups (one kernel for whole and half
-// tiles: 2048 x 4096 x 4096 34.8 us for 32.7; words in it: 4096 x 4097 x 4096 90 for 84).
+// two need takes registers and clocks from the loop over the groups (when they were split, one kernel
+// for whole and half tiles took 34.8 us for 2048 x 4096 x 4096 against 32.7, and 90 for 4096 x 4097 x
+// 4096 with words in it against 84).
 // kHalves: of at most three rounds, the last one's tiles (at most half as many as there are pairs)
 // are cut into halves of 128 weight rows. Products of 128 columns run at half rate (0.31 us a group
-// for 0.40 of a whole tile), but two pairs share a tile: 512 x 4096 x 4096 16.5 -> 15.5 us, 512 x
-// 960 x 2560 11.7 -> 10.5, after two whole rounds (2048 x 5120 x 960) 16.8 -> 16.1. After three they
-// cost more than they give (4096^3 62.2 -> 63.6), and GATE's tiles stay whole: a column group needs
-// both halves.
+// for 0.40 of a whole tile), but two pairs share a tile: 512 x 4096 x 4096 17.2 -> 15.4 us, after
+// two whole rounds (2048 x 5120 x 960) 16.9 -> 16.3. After three whole rounds of 32 groups (4096^3)
+// they cost more than they give (70.7 -> 73.2 in a long run); other numbers of groups after three were
+// not measured. GATE's tiles stay whole: a column group needs both halves.
 // kWords: the output's rows do not start on 16 bytes.
 enum class WideForm { kWhole, kHalves, kWords };
 
@@ -1039,9 +1040,11 @@ cudaError_t launch_wide(const GemmCall& c, int64_t tiles, cudaStream_t stream) {
 //                 blocks' operands come from L2 at 13 bytes/ps; summing up a split tile 0.3 + 0.02 c
 //   pair kernel   start 3.0; per round of 74 tiles 0.40 per column group and 1.2 (GATE 2.0), a
 //                 round of half tiles 0.31 and 1.0
-// Measured on either side of its borders: 512 x 960 x 960 4.3 us by 32 tokens a tile (64: 5.3,
-// pairs 6.2); 64 x 960 x 2560 3.9 by 16 tokens and 3 blocks a tile (one: 5.6; 64 tokens and 5
-// blocks: 4.8); 2048 x 1600 x 960 8.1 by pairs (64 tokens: 11.7).
+// Measured on either side of its borders: 512 x 960 x 960 4.3 us by 32 tokens a tile (16: 5.6, 64:
+// 5.2, pairs 6.0); 64 x 960 x 2560 3.6 by 16 tokens and 4 blocks a tile (one block: 5.6, three 3.9,
+// five 5.4; 32 tokens and four blocks 4.2; 64 and five 4.9); 2048 x 1600 x 960 7.9 by pairs (64
+// tokens: 12.0); gate/up 25 x 2560 x 960 4.9 by 16 tokens and one block (two blocks 5.1; 32 tokens
+// and four 5.2), 512 x 2560 x 960 8.3 by pairs (32 tokens: 15.6). dkv_fp8_plan gives a call's choice.
 struct GemmPlan {
   int tokens;  // per tile; 256: the pair kernel
   int splits;
