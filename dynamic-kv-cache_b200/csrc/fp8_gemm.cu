@@ -21,8 +21,9 @@
 //
 // fp8_wide_kernel (many tokens) is described below: 4096^3 64.5 us (76 in a long run of calls, under
 // the power cap), 2.13 PFLOP/s, 65 % of twice the measured bf16 rate (a plain library product of
-// these e4m3 matrices, without block scales: 49.5 us), bound by the round trip of an accumulator between the tensor cores and the threads
-// that scale it, and by 3.46 tiles per pair of SMs taking the time of 4.
+// these e4m3 matrices, without block scales: 49.5 us), bound by the round trip of an accumulator
+// between the tensor cores and the threads that scale it, and by 3.46 tiles per pair of SMs taking
+// the time of 4.
 //
 // GATE computes two products with the same rows, G and U, and writes silu(g) * u as e4m3
 // rows: a tile of 128 intermediate columns is exactly one column group of the next product,
